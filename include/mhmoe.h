@@ -102,6 +102,36 @@ MHMOE_API int mhmoe_topk(const float* logits, const float* expert_bias, int H, i
                int num_virtual_group, int topk_virtual_group, int route_norm, float norm_eps, float route_scale,
                float* probs, int64_t* idx, void* stream);
 
+/* Element types of the entry points that take one (x_dtype, y_dtype, ...). */
+typedef enum { MHMOE_F32 = 0, MHMOE_BF16 = 1, MHMOE_F16 = 2 } mhmoe_dtype;
+
+/* Expert routing with expert groups, masked experts and masked tokens (no counterpart in the
+ * reference: its virtual groups, mhmoe_topk, read the experts of the other groups as 0).
+ * logits [H, S, E] of `dtype` with element strides (any, 0 included; unit stride over E).
+ * An expert is masked where its logit or its bias is -inf; a token where token_mask (uint8
+ * [H, S], row stride mask_stride_h; optional) is 0.  Scores: softmax (0) or sigmoid (1).
+ * Selection keys: score + expert_bias (fp32 [H*E]), or the logits without a bias, compared
+ * as 64-bit values; NaN ranks below every number.  groups > 1: only the `topk_groups` groups
+ * with the largest sum of their two best unmasked score + bias stay.  Ties go to the lower
+ * id.  weights fp32 [H, S, K] = route_scale * score / max(sum of the K scores, norm_eps)
+ * (route_norm) or route_scale * score; idx int64 [H, S, K], -1 with weight 0 where no expert
+ * is left.  saved (optional, fp32 [H, S, K]) is what mhmoe_route_experts_bwd needs.
+ * E <= 1024, K <= 32, groups <= 64, K <= topk_groups * E / groups. */
+MHMOE_API int mhmoe_route_experts(const void* logits, int dtype, int64_t stride_h, int64_t stride_s,
+                                  const float* expert_bias, const uint8_t* token_mask, int64_t mask_stride_h, int H,
+                                  int S, int E, int K, int score_func, int groups, int topk_groups, int route_norm,
+                                  float norm_eps, float route_scale, float* weights, int64_t* idx, float* saved,
+                                  void* stream);
+
+/* Gradient of mhmoe_route_experts' weights with respect to the logits: grad_w fp32 [H, S, K]
+ * (element strides, unit over K), idx and saved as the forward wrote them; grad_logits
+ * [H, S, E] of `dtype`, contiguous, written whole.  The logits are read for softmax scores
+ * only (else NULL will do).  The expert bias takes part in the selection alone and has no gradient. */
+MHMOE_API int mhmoe_route_experts_bwd(const void* logits, int dtype, int64_t stride_h, int64_t stride_s, int H, int S,
+                                      int E, int K, int score_func, int route_norm, float norm_eps, float route_scale,
+                                      const float* grad_w, int64_t grad_stride_h, int64_t grad_stride_s,
+                                      const int64_t* idx, const float* saved, void* grad_logits, void* stream);
+
 /* ───────────────────────── permutation ───────────────────────── */
 
 /* Scratch bytes for mhmoe_global_sort (int32 chunk histograms). */
@@ -199,6 +229,55 @@ MHMOE_API int mhmoe_ffn_nvfp4_quantized(const uint8_t* xq, int64_t xq_pitch, con
                                         const int32_t* tok_rows, const int32_t* tok_offsets, int k_fixed,
                                         void* workspace, void* y, int64_t y_stride, int* dev_status,
                                         uint64_t timeout_ns, void* const* stage_events, void* stream);
+
+/* ───────────────────────── MXFP4 (E2M1 values, one E8M0 scale per 32) ─────────────────────────
+ * No counterpart in the reference.  A matrix [rows, cols] is packed bytes [rows, cols_p/2] (low
+ * nibble = even column, cols_p = cols rounded up to 128, padding 0) and scale bytes in 512-byte
+ * atoms of 128 rows x 128 columns: scale (row, block c) at ((row/128) * cols_p/128 + c/4) * 512 +
+ * (row%32)*16 + (row%128/32)*4 + c%4.  n matrices follow one another, each with
+ * ceil(rows/128) * cols_p/128 atoms.  data and scales are 16-byte aligned. */
+
+/* Quantise x [n, rows, cols] (element strides, unit over cols).  Per row and 32 columns:
+ * rounding 0 (floor): scale 2^(floor(log2 amax) - 2), larger values saturate at 6 * scale;
+ * 1 (ceil): the smallest power of two with amax <= 6 * scale.  Values round to nearest even.  A
+ * block that holds NaN or infinity becomes NaN (scale byte 255, codes 0). */
+MHMOE_API int mhmoe_mxfp4_quantize(const void* x, int x_dtype, int64_t stride_n, int64_t stride_row, int64_t n,
+                                   int64_t rows, int64_t cols, int rounding, uint8_t* data, uint8_t* scales,
+                                   void* stream);
+
+/* out [n, rows, cols] (contiguous) = the values of an MXFP4 matrix, rounded once to out_dtype
+ * (exact in fp32; in bf16 too, overflow apart). */
+MHMOE_API int mhmoe_mxfp4_dequantize(const uint8_t* data, const uint8_t* scales, int64_t n, int64_t rows, int64_t cols,
+                                     int out_dtype, void* out, void* stream);
+
+/* Scratch bytes of the two products below: x_rows activation rows, R output rows, n weight
+ * matrices [N, cols] (n = 1 and R = x_rows for mhmoe_mxfp4_linear). */
+MHMOE_API size_t mhmoe_mxfp4_workspace_bytes(int64_t x_rows, int64_t R, int n_experts, int N, int cols, int grouped);
+
+/* y [M, N'] = act(Q(x) W^T + bias) with W an MXFP4 matrix [N, cols], sums in fp32, one rounding to
+ * y_dtype.  x [M, cols] of x_dtype with row stride x_stride, quantised on the way (`rounding`),
+ * or already MXFP4 (x NULL, x_data / x_scales).  bias fp32 [N] or NULL.  activation 0: none,
+ * N' = N; 1: SwiGLU7 over column pairs (even gate, odd up), N' = N/2.  y_stride: row stride. */
+MHMOE_API int mhmoe_mxfp4_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_data,
+                                 const uint8_t* x_scales, int64_t M, int cols, int rounding, const uint8_t* w_data,
+                                 const uint8_t* w_scales, int N, const float* bias, int activation, void* workspace,
+                                 void* y, int y_dtype, int64_t y_stride, int* dev_status, uint64_t timeout_ns,
+                                 void* stream);
+
+/* The same product per expert over rows sorted by expert (mhmoe_global_sort): row r of expert e,
+ * expert_offsets[e] <= r < expert_offsets[e+1], gives
+ *   y[r] = row_weights[r] * act(Q(x[gather_ids[r]]) W_e^T + bias_e)
+ * with W n_experts matrices [N, cols], bias fp32 [n_experts, N] or NULL, row_weights fp32 [R] or
+ * NULL, gather_ids int32 [R] or NULL (row r of x itself; then x_rows >= R).  R is the rows y
+ * has; the rows from expert_offsets[n_experts] on are not computed: left as they are, or set to
+ * 0 with zero_tail.  Offsets outside [0, R] are clipped and a gather id outside [0, x_rows) reads
+ * as a row of zeros; both, and offsets that decrease, record MHMOE_ERR_ARGS in dev_status. */
+MHMOE_API int mhmoe_mxfp4_expert_linear(const void* x, int x_dtype, int64_t x_stride, int64_t x_rows, int cols,
+                                        int rounding, const uint8_t* w_data, const uint8_t* w_scales, int n_experts,
+                                        int N, const int64_t* expert_offsets, const int32_t* gather_ids, int64_t R,
+                                        const float* row_weights, const float* bias, int activation, void* workspace,
+                                        void* y, int y_dtype, int64_t y_stride, int zero_tail, int* dev_status,
+                                        uint64_t timeout_ns, void* stream);
 
 /* ───────────────────────── building blocks (tests, EP) ───────────────────────── */
 

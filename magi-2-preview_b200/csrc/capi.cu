@@ -9,6 +9,7 @@
 #include <string>
 
 #include "kernels.cuh"
+#include "mxfp4.cuh"
 
 namespace {
 
@@ -284,6 +285,128 @@ int mhmoe_ffn_nvfp4_quantized(const uint8_t* xq, int64_t xq_pitch, const uint8_t
   if (rc == MHMOE_ERR_LAUNCH) return fail_cuda(ce, "ffn_nvfp4_quantized");
   if (rc == MHMOE_ERR_DRIVER) g_last_error = "cuTensorMapEncodeTiled failed";
   return rc;
+}
+
+static bool known_dtype(int d) { return d == MHMOE_F32 || d == MHMOE_BF16 || d == MHMOE_F16; }
+
+int mhmoe_route_experts(const void* logits, int dtype, int64_t stride_h, int64_t stride_s, const float* expert_bias,
+                        const uint8_t* token_mask, int64_t mask_stride_h, int H, int S, int E, int K, int score_func,
+                        int groups, int topk_groups, int route_norm, float norm_eps, float route_scale, float* weights,
+                        int64_t* idx, float* saved, void* stream) {
+  MHMOE_REQUIRE(known_dtype(dtype) && (score_func == 0 || score_func == 1));
+  MHMOE_REQUIRE(H > 0 && S >= 0 && E > 0 && E <= 1024 && K > 0 && K <= 32 && K <= E);
+  MHMOE_REQUIRE(groups > 0 && groups <= 64 && E % groups == 0 && topk_groups > 0 && topk_groups <= groups);
+  MHMOE_REQUIRE(K <= topk_groups * (E / groups));
+  MHMOE_REQUIRE((int64_t)H * S < (int64_t)1 << 31);
+  MHMOE_REQUIRE(S == 0 || (logits && weights && idx));
+  MHMOE_CHECK_ARCH();
+  if (S == 0) return MHMOE_OK;
+  const RouteArgs a{logits, dtype, stride_h, stride_s, expert_bias, token_mask, mask_stride_h, H, S, E, K, score_func,
+                    groups, topk_groups, route_norm, norm_eps, route_scale};
+  const cudaError_t e = launch_route_experts(a, weights, idx, saved, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MHMOE_OK : fail_cuda(e, "route_experts");
+}
+
+int mhmoe_route_experts_bwd(const void* logits, int dtype, int64_t stride_h, int64_t stride_s, int H, int S, int E,
+                            int K, int score_func, int route_norm, float norm_eps, float route_scale,
+                            const float* grad_w, int64_t grad_stride_h, int64_t grad_stride_s, const int64_t* idx,
+                            const float* saved, void* grad_logits, void* stream) {
+  MHMOE_REQUIRE(known_dtype(dtype) && (score_func == 0 || score_func == 1));
+  MHMOE_REQUIRE(H > 0 && S >= 0 && E > 0 && E <= 1024 && K > 0 && K <= 32 && K <= E);
+  MHMOE_REQUIRE((int64_t)H * S < (int64_t)1 << 31);
+  MHMOE_REQUIRE(S == 0 || (grad_w && idx && saved && grad_logits && (logits || score_func == 1)));
+  MHMOE_CHECK_ARCH();
+  if (S == 0) return MHMOE_OK;
+  const RouteArgs a{logits, dtype, stride_h, stride_s, nullptr, nullptr, 0, H, S, E, K, score_func, 1, 1, route_norm,
+                    norm_eps, route_scale};
+  const cudaError_t e = launch_route_experts_bwd(a, grad_w, grad_stride_h, grad_stride_s, idx, saved, grad_logits,
+                                                 static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MHMOE_OK : fail_cuda(e, "route_experts_bwd");
+}
+
+int mhmoe_mxfp4_quantize(const void* x, int x_dtype, int64_t stride_n, int64_t stride_row, int64_t n, int64_t rows,
+                         int64_t cols, int rounding, uint8_t* data, uint8_t* scales, void* stream) {
+  MHMOE_REQUIRE(known_dtype(x_dtype) && (rounding == 0 || rounding == 1));
+  MHMOE_REQUIRE(n >= 0 && rows >= 0 && cols > 0 && cols < (int64_t)1 << 30);
+  if (n * rows > 0) MHMOE_REQUIRE(x && data && scales && aligned16(data) && aligned16(scales));
+  MHMOE_CHECK_ARCH();
+  if (n * rows == 0) return MHMOE_OK;
+  const cudaError_t e = launch_mx_quantize(x, x_dtype, stride_n, stride_row, n, rows, cols, rounding == 1, data, scales,
+                                           static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MHMOE_OK : fail_cuda(e, "mxfp4_quantize");
+}
+
+int mhmoe_mxfp4_dequantize(const uint8_t* data, const uint8_t* scales, int64_t n, int64_t rows, int64_t cols,
+                           int out_dtype, void* out, void* stream) {
+  MHMOE_REQUIRE(known_dtype(out_dtype) && n >= 0 && rows >= 0 && cols > 0 && cols < (int64_t)1 << 30);
+  if (n * rows > 0) MHMOE_REQUIRE(out && data && scales && aligned16(data) && aligned16(scales));
+  MHMOE_CHECK_ARCH();
+  if (n * rows == 0) return MHMOE_OK;
+  const cudaError_t e =
+      launch_mx_dequantize(data, scales, n, rows, cols, out_dtype, out, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? MHMOE_OK : fail_cuda(e, "mxfp4_dequantize");
+}
+
+size_t mhmoe_mxfp4_workspace_bytes(int64_t x_rows, int64_t R, int n_experts, int N, int cols, int grouped) {
+  if (x_rows < 0 || R < 0 || n_experts <= 0 || N <= 0 || cols <= 0) return 0;
+  return mx_product_workspace_bytes(x_rows, R, n_experts, N, cols, grouped != 0);
+}
+
+static int mx_entry(const MxProduct& p, void* workspace, void* stream, const char* what) {
+  cudaError_t ce = cudaSuccess;
+  const int rc = mx_product(p, workspace, static_cast<cudaStream_t>(stream), &ce);
+  if (rc == MHMOE_ERR_LAUNCH) return fail_cuda(ce, what);
+  if (rc == MHMOE_ERR_DRIVER) g_last_error = std::string("cuTensorMapEncodeTiled failed (") + what + ")";
+  return rc;
+}
+
+// Limits shared by the products: sizes that the kernels' 32-bit coordinates hold.
+static bool mx_sizes_ok(int64_t x_rows, int64_t R, int n, int N, int cols) {
+  return x_rows >= 0 && R >= 0 && n > 0 && n <= 12288 && N > 0 && N <= 1 << 20 && cols > 0 && cols <= 1 << 20 &&
+         x_rows < (int64_t)1 << 30 && R < (int64_t)1 << 30 && (int64_t)n * N < (int64_t)1 << 31;
+}
+
+int mhmoe_mxfp4_linear(const void* x, int x_dtype, int64_t x_stride, const uint8_t* x_data, const uint8_t* x_scales,
+                       int64_t M, int cols, int rounding, const uint8_t* w_data, const uint8_t* w_scales, int N,
+                       const float* bias, int activation, void* workspace, void* y, int y_dtype, int64_t y_stride,
+                       int* dev_status, uint64_t timeout_ns, void* stream) {
+  MHMOE_REQUIRE(known_dtype(y_dtype) && known_dtype(x_dtype) && (rounding == 0 || rounding == 1));
+  MHMOE_REQUIRE(mx_sizes_ok(M, M, 1, N, cols));
+  MHMOE_REQUIRE(activation == 0 || (activation == 1 && N % 2 == 0));
+  MHMOE_REQUIRE(w_data && w_scales && aligned16(w_data) && aligned16(w_scales));
+  if (M > 0) {
+    MHMOE_REQUIRE(y && y_stride >= (activation ? N / 2 : N));
+    MHMOE_REQUIRE((x && workspace && aligned16(workspace)) ||
+                  (!x && x_data && x_scales && aligned16(x_data) && aligned16(x_scales)));
+  }
+  MHMOE_CHECK_ARCH();
+  if (M == 0) return MHMOE_OK;
+  const MxProduct p{x,       x_dtype, x_stride, M, rounding == 1, x ? nullptr : x_data, x ? nullptr : x_scales,
+                    w_data,  w_scales, 1, N, cols, nullptr, nullptr, M, nullptr, bias, activation, y, y_dtype, y_stride,
+                    false, dev_status, timeout_ns};
+  return mx_entry(p, workspace, stream, "mxfp4_linear");
+}
+
+int mhmoe_mxfp4_expert_linear(const void* x, int x_dtype, int64_t x_stride, int64_t x_rows, int cols, int rounding,
+                              const uint8_t* w_data, const uint8_t* w_scales, int n_experts, int N,
+                              const int64_t* expert_offsets, const int32_t* gather_ids, int64_t R,
+                              const float* row_weights, const float* bias, int activation, void* workspace, void* y,
+                              int y_dtype, int64_t y_stride, int zero_tail, int* dev_status, uint64_t timeout_ns,
+                              void* stream) {
+  MHMOE_REQUIRE(known_dtype(y_dtype) && known_dtype(x_dtype) && (rounding == 0 || rounding == 1));
+  MHMOE_REQUIRE(mx_sizes_ok(x_rows, R, n_experts, N, cols));
+  MHMOE_REQUIRE(activation == 0 || (activation == 1 && N % 2 == 0));
+  MHMOE_REQUIRE(w_data && w_scales && aligned16(w_data) && aligned16(w_scales) && expert_offsets);
+  if (R > 0) {
+    MHMOE_REQUIRE(y && y_stride >= (activation ? N / 2 : N) && workspace && aligned16(workspace));
+    MHMOE_REQUIRE((x || x_rows == 0) && (gather_ids || x_rows >= R));
+  }
+  MHMOE_CHECK_ARCH();
+  if (R == 0) return MHMOE_OK;
+  const MxProduct p{x,       x_dtype, x_stride, x_rows, rounding == 1, nullptr, nullptr,
+                    w_data,  w_scales, n_experts, N, cols, expert_offsets, gather_ids, R, row_weights, bias, activation,
+                    y, y_dtype, y_stride, zero_tail != 0, dev_status, timeout_ns};
+  return mx_entry(p, workspace, stream, "mxfp4_expert_linear");
 }
 
 int mhmoe_quant_tokens(const void* x, int64_t x_stride_s, int64_t x_stride_h, int S, int H, int dh, uint8_t* xq,

@@ -1,0 +1,132 @@
+// MXFP4 quantisation and its inverse.
+//
+// quantise: per row and per 32 columns, a = max |x|, e from mx_scale_byte, values
+// E2M1(x * 2^-e) rounded to nearest even and saturated at 6.  x * 2^-e is exact in fp32 (a power
+// of two; results below the E2M1 range round to 0 either way), so the codes are the
+// definition's for every input type.
+//
+// Both kernels are bound by HBM: 2 or 4 bytes an element one way, 17/32 of a byte the other.
+#include "mxfp4.cuh"
+
+namespace mhmoe {
+
+constexpr int MXQ_THREADS = 256;
+
+// A thread holds 8 columns (one 4-B word of codes); 4 neighbours make a block, 16 an atom
+// column of 128 (one 4-B word of scales).  Items are (matrix, row, atom column) with the
+// rows of each matrix counted to a multiple of 128, so that every scale byte is written.
+template <int DT>
+__global__ void __launch_bounds__(MXQ_THREADS)
+    mx_quantize_kernel(const typename MxType<DT>::T* __restrict__ x, int64_t stride_n, int64_t stride_row,
+                       int64_t rows, int64_t rows_p, uint32_t cols, uint32_t katoms, int64_t items, bool ceil,
+                       bool vec_ok, uint8_t* __restrict__ data, uint8_t* __restrict__ sf) {
+  pdl_wait();
+  pdl_trigger();
+  const int sub = threadIdx.x & 15;
+  for (int64_t it = (int64_t)blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
+       it += (int64_t)gridDim.x * (MXQ_THREADS / 16)) {
+    const uint32_t ka = (uint32_t)(it % katoms);
+    const int64_t rr = it / katoms;
+    const int64_t b = rr / rows_p, row = rr % rows_p;
+    const uint32_t c0 = ka * 128 + sub * 8;
+    float v[8] = {};
+    const bool live = row < rows;
+    if (live && c0 < cols)
+      mx_load8(x + b * stride_n + row * stride_row + c0, vec_ok && c0 + 8 <= cols, (int)min(8u, cols - c0), v);
+    uint32_t a = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+    // the 16 lanes of an item stay together: items split warps into halves
+    const uint32_t mask = 0xffffu << (threadIdx.x & 16);
+    a = max(a, __shfl_xor_sync(mask, a, 1));
+    a = max(a, __shfl_xor_sync(mask, a, 2));
+    const uint32_t s = mx_scale_byte(a, ceil);
+    uint32_t w = 0;
+    if (s != 255u) {
+      const float f = mx_inv_scale(s);
+      w = cvt_e2m1x8(v[0] * f, v[1] * f, v[2] * f, v[3] * f, v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+    }
+    uint32_t sw = s << (8 * (sub >> 2));
+    sw |= __shfl_xor_sync(mask, sw, 4);
+    sw |= __shfl_xor_sync(mask, sw, 8);
+    if (live) *reinterpret_cast<uint32_t*>(data + (b * rows + row) * (int64_t)katoms * 64 + ka * 64 + sub * 4) = w;
+    if (sub == 0)
+      *reinterpret_cast<uint32_t*>(sf + (uint64_t)b * (rows_p >> 7) * katoms * 512 + mx_sf_offset(row, ka * 4, katoms)) =
+          sw;
+  }
+}
+
+template <int DT>
+__global__ void __launch_bounds__(MXQ_THREADS)
+    mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ sf, int64_t rows,
+                         int64_t rows_p, uint32_t cols, uint32_t katoms, int64_t items, bool vec_ok,
+                         typename MxType<DT>::T* __restrict__ out) {
+  pdl_wait();
+  pdl_trigger();
+  using T = typename MxType<DT>::T;
+  const int sub = threadIdx.x & 15;
+  for (int64_t it = (int64_t)blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
+       it += (int64_t)gridDim.x * (MXQ_THREADS / 16)) {
+    const uint32_t ka = (uint32_t)(it % katoms);
+    const int64_t rr = it / katoms;
+    const int64_t b = rr / rows, row = rr % rows;
+    const uint32_t c0 = ka * 128 + sub * 8;
+    if (c0 >= cols) continue;
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(data + rr * (int64_t)katoms * 64 + ka * 64 + sub * 4));
+    const float s = mx_scale_value(__ldg(sf + (uint64_t)b * (rows_p >> 7) * katoms * 512 +
+                                         mx_sf_offset(row, ka * 4 + (sub >> 2), katoms)));
+    float v[8];
+    mx_decode8(w, v);
+    T* o = out + rr * (int64_t)cols + c0;
+    if (vec_ok && c0 + 8 <= cols) {
+      __align__(16) T t[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx_store(&t[i], v[i] * s);
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(t)[i];
+    } else {
+      for (uint32_t i = 0; i < min(8u, cols - c0); ++i) mx_store(o + i, v[i] * s);
+    }
+  }
+}
+
+static unsigned mx_grid(int64_t items) {
+  const int64_t blocks = (items + MXQ_THREADS / 16 - 1) / (MXQ_THREADS / 16);
+  return (unsigned)std::min<int64_t>(blocks, (int64_t)num_sms() * 64);
+}
+
+cudaError_t launch_mx_quantize(const void* x, int dtype, int64_t stride_n, int64_t stride_row, int64_t n,
+                               int64_t rows, int64_t cols, bool ceil, uint8_t* data, uint8_t* sf, cudaStream_t st) {
+  const int64_t rows_p = (rows + 127) / 128 * 128, katoms = mx_padded_cols(cols) / 128;
+  const int64_t items = n * rows_p * katoms;
+  if (items == 0) return cudaSuccess;
+  const int64_t esz = dtype == DT_F32 ? 4 : 2;
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride_n * esz % 16 == 0 && stride_row * esz % 16 == 0;
+#define MX_Q(DT)                                                                                                  \
+  MHMOE_LAUNCH_PDL(mx_quantize_kernel<DT>, mx_grid(items), MXQ_THREADS, 0, st,                                    \
+                   static_cast<const MxType<DT>::T*>(x), stride_n, stride_row, rows, rows_p, (uint32_t)cols,      \
+                   (uint32_t)katoms, items, ceil, vec, data, sf)
+  if (dtype == DT_F32) MX_Q(DT_F32);
+  else if (dtype == DT_BF16) MX_Q(DT_BF16);
+  else MX_Q(DT_F16);
+#undef MX_Q
+  return cudaGetLastError();
+}
+
+cudaError_t launch_mx_dequantize(const uint8_t* data, const uint8_t* sf, int64_t n, int64_t rows, int64_t cols,
+                                 int dtype, void* out, cudaStream_t st) {
+  const int64_t rows_p = (rows + 127) / 128 * 128, katoms = mx_padded_cols(cols) / 128;
+  const int64_t items = n * rows * katoms;
+  if (items == 0) return cudaSuccess;
+  const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && cols * (dtype == DT_F32 ? 4 : 2) % 16 == 0;
+#define MX_D(DT)                                                                                                  \
+  MHMOE_LAUNCH_PDL(mx_dequantize_kernel<DT>, mx_grid(items), MXQ_THREADS, 0, st, data, sf, rows, rows_p,          \
+                   (uint32_t)cols, (uint32_t)katoms, items, vec, static_cast<MxType<DT>::T*>(out))
+  if (dtype == DT_F32) MX_D(DT_F32);
+  else if (dtype == DT_BF16) MX_D(DT_BF16);
+  else MX_D(DT_F16);
+#undef MX_D
+  return cudaGetLastError();
+}
+
+}  // namespace mhmoe

@@ -31,6 +31,17 @@ SIGNATURES: dict[str, tuple] = {
     "mhmoe_route": (i32, [vp, i64, i64, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp, i32, f32, f32, vp, vp, vp,
                           vp, vp]),
     "mhmoe_topk": (i32, [vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp, vp, vp]),
+    "mhmoe_route_experts": (i32, [vp, i32, i64, i64, vp, vp, i64, i32, i32, i32, i32, i32, i32, i32, i32, f32, f32, vp,
+                                  vp, vp, vp]),
+    "mhmoe_route_experts_bwd": (i32, [vp, i32, i64, i64, i32, i32, i32, i32, i32, i32, f32, f32, vp, i64, i64, vp, vp,
+                                      vp, vp]),
+    "mhmoe_mxfp4_quantize": (i32, [vp, i32, i64, i64, i64, i64, i64, i32, vp, vp, vp]),
+    "mhmoe_mxfp4_dequantize": (i32, [vp, vp, i64, i64, i64, i32, vp, vp]),
+    "mhmoe_mxfp4_workspace_bytes": (sz, [i64, i64, i32, i32, i32, i32]),
+    "mhmoe_mxfp4_linear": (i32, [vp, i32, i64, vp, vp, i64, i32, i32, vp, vp, i32, vp, i32, vp, vp, i32, i64, vp, u64,
+                                 vp]),
+    "mhmoe_mxfp4_expert_linear": (i32, [vp, i32, i64, i64, i32, i32, vp, vp, i32, i32, vp, vp, i64, vp, vp, i32, vp, vp,
+                                        i32, i64, i32, vp, u64, vp]),
     "mhmoe_global_sort_workspace_bytes": (sz, [i32, i32, i32, i32]),
     "mhmoe_global_sort": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp, vp]),
     "mhmoe_global_sort_noalloc": (i32, [vp, vp, i32, i32, i32, i32, vp, vp, vp, vp, vp, vp]),
@@ -89,6 +100,10 @@ def lib() -> C.CDLL:
             fn.argtypes = args
         _lib = h
     return _lib
+
+
+# element types of the entry points that take one (mhmoe_dtype)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class MHMoEError(RuntimeError):

@@ -185,3 +185,104 @@ def route_fused(x_heads: torch.Tensor, planes: torch.Tensor, nsplit: int, num_ex
             float(route_scale), probs.data_ptr(), idx.data_ptr(), _lib.ptr(logits),
             _lib.device_status(dev).data_ptr(), _lib.stream_ptr(dev)), "route")
     return (probs, idx, logits) if return_logits else (probs, idx)
+
+
+# ───────────────────────── routing with expert groups, masks and gradients ─────────────────────────
+
+class _RouteExperts(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, mask, top_k, score_func, groups, keep, route_norm, norm_eps, route_scale):
+        H, S, E = logits.shape
+        dev = logits.device
+        weights = torch.empty(H, S, top_k, dtype=torch.float32, device=dev)
+        idx = torch.empty(H, S, top_k, dtype=torch.int64, device=dev)
+        saved = torch.empty(H, S, top_k, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().mhmoe_route_experts(
+                logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0), logits.stride(1), _lib.ptr(bias),
+                _lib.ptr(mask), 0 if mask is None else mask.stride(0), H, S, E, top_k, score_func, groups, keep,
+                route_norm, norm_eps, route_scale, weights.data_ptr(), idx.data_ptr(), _lib.ptr(saved),
+                _lib.stream_ptr(dev)), "route_experts")
+        ctx.mark_non_differentiable(idx)
+        if saved is not None:
+            # sigmoid gradients need the chosen experts' logits only, which `saved` holds
+            ctx.save_for_backward(logits if score_func == 0 else None, idx, saved)
+            ctx.meta = (logits.dtype, E, score_func, route_norm, norm_eps, route_scale)
+        return weights, idx
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_w, _grad_idx):
+        logits, idx, saved = ctx.saved_tensors
+        dtype, E, score_func, route_norm, norm_eps, route_scale = ctx.meta
+        H, S, K = idx.shape
+        g = grad_w.float()
+        if K > 1 and g.stride(2) != 1:
+            g = g.contiguous()
+        dev = idx.device
+        out = torch.empty(H, S, E, dtype=dtype, device=dev)
+        with torch.cuda.device(dev):
+            _lib.check(_lib.lib().mhmoe_route_experts_bwd(
+                _lib.ptr(logits), _lib.DTYPES[dtype], 0 if logits is None else logits.stride(0),
+                0 if logits is None else logits.stride(1), H, S, E, K, score_func, route_norm, norm_eps, route_scale,
+                g.data_ptr(), g.stride(0), g.stride(1), idx.data_ptr(), saved.data_ptr(), out.data_ptr(),
+                _lib.stream_ptr(dev)), "route_experts backward")
+        return out, None, None, None, None, None, None, None, None, None
+
+
+def route_experts(
+    logits: torch.Tensor,
+    top_k: int,
+    score_func: TopKScoreFunc = "softmax",
+    expert_bias: torch.Tensor | None = None,
+    num_groups: int = 1,
+    topk_groups: int = 1,
+    route_norm: bool = True,
+    norm_eps: float = 1e-12,
+    route_scale: float = 1.0,
+    token_mask: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Trainable top-k gating of logits [H, S, E] (fp32, bf16 or fp16, any outer strides).
+
+    Returns (weights fp32 [H, S, K], indices int64 [H, S, K]).  With s the softmax or sigmoid
+    scores:
+
+    * candidates are ranked by ``s + expert_bias`` ([H, E] or [H*E], fp32), or by the logits
+      without a bias, as 64-bit values (no dependence on how 32-bit scores round); ties go to
+      the lower id, NaN ranks below every number;
+    * ``num_groups`` > 1 splits the E experts into equal consecutive groups and keeps the
+      ``topk_groups`` groups whose two best candidates have the largest sum; unlike
+      ``compute_topk_probs_and_indices``'s virtual groups, the other groups' experts are
+      never chosen;
+    * an expert whose logit or bias is -inf is never chosen; where fewer than ``top_k`` experts
+      are left, the remaining slots hold index -1 and weight 0 (the global sort skips them);
+    * ``token_mask`` (bool [S] or [H, S]): tokens that are False get -1 and 0 throughout, and
+      their logits (NaN included) are not looked at;
+    * weights are ``route_scale * s / max(sum of the chosen s, norm_eps)``, or
+      ``route_scale * s`` without ``route_norm``.
+
+    The weights are differentiable in the logits (first order); the bias only steers the
+    selection and gets no gradient.  E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not
+    exceed the experts of ``topk_groups`` groups (``ValueError``).
+    """
+    if score_func not in score_func_name2id_map:
+        raise ValueError(f"Unknown score_func: {score_func}")
+    if logits.dim() != 3 or logits.dtype not in _lib.DTYPES:
+        raise ValueError(f"logits must be [H, S, E] in fp32, bf16 or fp16, got {tuple(logits.shape)} {logits.dtype}")
+    H, S, E = logits.shape
+    _lib.require_cuda(logits, expert_bias, token_mask)
+    for name, t in (("expert_bias", expert_bias), ("token_mask", token_mask)):
+        if t is not None and t.device != logits.device:
+            raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
+    bias = mask = None
+    if expert_bias is not None:
+        if expert_bias.numel() != H * E:
+            raise ValueError(f"expert_bias must hold H*E = {H * E} values, got {tuple(expert_bias.shape)}")
+        bias = expert_bias.detach().reshape(H, E).float().contiguous()
+    if token_mask is not None:
+        if token_mask.dtype != torch.bool or tuple(token_mask.shape) not in ((S,), (H, S)):
+            raise ValueError(f"token_mask must be bool [S] or [H, S], got {tuple(token_mask.shape)} {token_mask.dtype}")
+        mask = token_mask.contiguous().view(torch.uint8).expand(H, S)
+    x = logits if E == 1 or logits.stride(2) == 1 else logits.contiguous()
+    return _RouteExperts.apply(x, bias, mask, int(top_k), score_func_name2id_map[score_func], int(num_groups),
+                               int(topk_groups), int(bool(route_norm)), float(norm_eps), float(route_scale))
