@@ -33,22 +33,9 @@ __global__ void __launch_bounds__(MXQ_THREADS)
     const bool live = row < rows;
     if (live && c0 < cols)
       mx_load8(x + b * stride_n + row * stride_row + c0, vec_ok && c0 + 8 <= cols, (int)min(8u, cols - c0), v);
-    uint32_t a = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+    uint32_t sw;
     // the 16 lanes of an item stay together: items split warps into halves
-    const uint32_t mask = 0xffffu << (threadIdx.x & 16);
-    a = max(a, __shfl_xor_sync(mask, a, 1));
-    a = max(a, __shfl_xor_sync(mask, a, 2));
-    const uint32_t s = mx_scale_byte(a, ceil);
-    uint32_t w = 0;
-    if (s != 255u) {
-      const float f = mx_inv_scale(s);
-      w = cvt_e2m1x8(v[0] * f, v[1] * f, v[2] * f, v[3] * f, v[4] * f, v[5] * f, v[6] * f, v[7] * f);
-    }
-    uint32_t sw = s << (8 * (sub >> 2));
-    sw |= __shfl_xor_sync(mask, sw, 4);
-    sw |= __shfl_xor_sync(mask, sw, 8);
+    const uint32_t w = mx_quantize8(v, ceil, sub, 0xffffu << (threadIdx.x & 16), sw);
     if (live) *reinterpret_cast<uint32_t*>(data + (b * rows + row) * (int64_t)katoms * 64 + ka * 64 + sub * 4) = w;
     if (sub == 0)
       *reinterpret_cast<uint32_t*>(sf + (uint64_t)b * (rows_p >> 7) * katoms * 512 + mx_sf_offset(row, ka * 4, katoms)) =

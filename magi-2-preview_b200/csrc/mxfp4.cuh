@@ -92,6 +92,27 @@ __device__ __forceinline__ float mx_scale_value(uint32_t b) {
   return __uint_as_float(b == 255u ? 0x7fc00000u : b << 23);
 }
 
+// Quantise the 8 values of a thread: four neighbouring threads hold a block of 32, sixteen (sub =
+// 0..15, all in `mask`) an atom column of 128.  Returns the packed codes; sw is the atom
+// column's four scale bytes, the same word in all sixteen.
+__device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], bool ceil, int sub, uint32_t mask, uint32_t& sw) {
+  uint32_t a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+  a = max(a, __shfl_xor_sync(mask, a, 1));
+  a = max(a, __shfl_xor_sync(mask, a, 2));
+  const uint32_t s = mx_scale_byte(a, ceil);
+  uint32_t w = 0;
+  if (s != 255u) {
+    const float f = mx_inv_scale(s);
+    w = cvt_e2m1x8(v[0] * f, v[1] * f, v[2] * f, v[3] * f, v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+  }
+  sw = s << (8 * (sub >> 2));
+  sw |= __shfl_xor_sync(mask, sw, 4);
+  sw |= __shfl_xor_sync(mask, sw, 8);
+  return w;
+}
+
 // Eight E2M1 values of a packed word (nibble i = value i) as fp32.
 __device__ __forceinline__ void mx_decode8(uint32_t w, float (&v)[8]) {
   uint32_t h[4];

@@ -2,175 +2,776 @@
 //
 // Every product of two E2M1 values and of two scales is exact in fp32, so the result is the
 // fp32 sum of exact terms, plus the epilogue's roundings: one to the output's type.
+//
+// Two launches.  The first quantises the activations (mx_quantize_kernel, or mx_group_kernel
+// for expert rows: gather, quantise, scale atoms per token tile, and in one extra block the list
+// of token tiles).  The second, mx_gemm_kernel, multiplies on the tensor cores
+// (tcgen05.mma kind::mxf4, fp32 accumulators in TMEM).
+//
+// A work item is (token tile, weight tile).  Two orientations share the main loop:
+//   wide   A = 128 token rows, B = 256 weight rows: the most math per operand byte
+//   flat   A = 128 weight rows, B = 16..128 token rows: a few tokens still fill the
+//          instruction's 128 lanes with weights, which is what a decode step streams
+// Warp roles: 0 TMA producer, 1 TMEM owner and MMA issuer, then the epilogue warps, last the
+// copier of scale atoms into TMEM (their own warp, so that copies run beside the MMAs).  One
+// stage is 256 columns (128 B a row) of both operands with their scale atoms.
 #include "mxfp4.cuh"
 
 namespace mhmoe {
 
 namespace {
 
-constexpr int SG_BM = 64, SG_BN = 64, SG_BK = 32;
+constexpr int MG_BM = 128;                  // rows of operand A
+constexpr int MG_BK = 256;                  // columns of a stage
+constexpr int MG_A_BYTES = MG_BM * MG_BK / 2;
+constexpr int MG_SFA_BYTES = 2 * 512;       // two atoms: 128 rows x 256 columns
+constexpr int MG_STG_BYTES = 2048;          // store staging per epilogue warp (wide): 32 rows x 64 B
+constexpr int MG_MISC_BYTES = 512;          // barriers, TMEM slot
+constexpr int MG_TMEM_COLS = 512;
 
-struct SimpleArgs {
-  const uint8_t* xq;
-  const uint8_t* xsf;
-  const uint8_t* w;
-  const uint8_t* wsf;
-  int n, N;
+template <bool FLAT, int BN>
+struct MgShape {
+  static constexpr int NBLK = (BN + 127) / 128;                 // 128-row atom blocks of operand B
+  static constexpr int B_BYTES = BN * MG_BK / 2;
+  static constexpr int SFB_BYTES = NBLK * MG_SFA_BYTES;
+  static constexpr int STAGE = MG_A_BYTES + B_BYTES + MG_SFA_BYTES + SFB_BYTES;
+  static constexpr int EPW = FLAT ? 4 : 8;                      // epilogue warps
+  static constexpr int STG = FLAT ? 0 : EPW * MG_STG_BYTES;
+  static constexpr int STAGES = FLAT ? (BN <= 16 ? 10 : BN <= 32 ? 9 : BN <= 64 ? 8 : 6) : 4;
+  static constexpr int SMEM = STAGES * STAGE + STG + MG_MISC_BYTES + 1024;
+  static constexpr int THREADS = 32 * (3 + EPW);
+  static constexpr int NACC = FLAT ? 2 : 1;                     // accumulators in TMEM
+  static constexpr int SF_COLS = 8 + 8 * NBLK;                  // TMEM columns of a stage's scales
+  static constexpr int SF_COL0 = NACC * BN;
+  static constexpr int SLOT = FLAT ? BN : MG_BM;                // token rows of a tile
+  static constexpr int WROWS = FLAT ? MG_BM : BN;               // weight rows of a tile
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(SF_COL0 + STAGES * SF_COLS <= MG_TMEM_COLS, "TMEM");
+};
+
+struct MgParams {
+  const uint8_t* sf_tok;      // scale atoms of the token tiles, one 128-row block per slot
+  const uint8_t* sf_w;
+  const int4* tiles;          // grouped: {expert, first row, rows, slot}; null: dense
+  const int* n_tiles;         // grouped: their number (device)
+  int max_tiles;
+  int64_t R;
+  int N, n_wt;
   uint32_t katoms;
-  const int64_t* offsets;
-  const int32_t* gather;
-  int64_t R, x_rows;
   const float* row_weights;
   const float* bias;
   int act;
+  void* y;
+  int y_dtype;
   int64_t y_stride;
+  bool y_vec;                 // 16-B stores are possible
+  int* status;
+  uint64_t timeout_ns;
+};
+
+struct MgTile {
+  int e, rows;
+  int64_t row0, slot;
+};
+
+template <int SLOT>
+__device__ __forceinline__ MgTile mg_tile(const MgParams& p, int tt) {
+  MgTile t;
+  if (p.tiles) {
+    const int4 v = __ldg(p.tiles + tt);
+    t.e = v.x;
+    t.row0 = v.y;
+    t.rows = v.z;
+    t.slot = v.w;
+  } else {
+    t.e = 0;
+    t.row0 = (int64_t)tt * SLOT;
+    t.rows = (int)min((int64_t)SLOT, p.R - t.row0);
+    t.slot = tt;
+  }
+  return t;
+}
+
+__device__ __forceinline__ uint32_t mg_pack16(float a, float b, bool half) {
+  if (half) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void mg_store(void* y, int dtype, int64_t at, float v) {
+  if (dtype == DT_F32) static_cast<float*>(y)[at] = v;
+  else if (dtype == DT_BF16) static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(v);
+  else static_cast<__half*>(y)[at] = __float2half_rn(v);
+}
+
+// Epilogue of 32 token rows (one a thread) x 128 accumulator columns: 64 B of outputs per row
+// go through the warp's staging (16-B chunks xor-swizzled over row pairs) and leave as whole
+// sectors, 8 rows a store.
+template <bool OUT32, bool SWIGLU>
+__device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, const uint32_t (&r)[128], int col0,
+                                                 int q, int lane, uint8_t* stg) {
+  constexpr int PER = OUT32 ? 16 : 32;              // outputs of a 64-B chunk
+  constexpr int ACC = SWIGLU ? 2 * PER : PER;       // accumulator columns behind them
+  const int n_out = SWIGLU ? p.N / 2 : p.N;
+  const int m = q * 32 + lane;
+  const float rw = p.row_weights && m < t.rows ? __ldg(p.row_weights + t.row0 + m) : 1.f;
+  const float* bias = p.bias ? p.bias + (int64_t)t.e * p.N : nullptr;
+  const bool half = p.y_dtype == DT_F16;
+#pragma unroll
+  for (int c = 0; c < 128 / ACC; ++c) {
+    const int a0 = col0 + c * ACC;                  // first weight row of the chunk
+    const int o0 = SWIGLU ? a0 / 2 : a0;
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      if constexpr (SWIGLU) {
+        float g = __uint_as_float(r[c * ACC + 2 * i]), u = __uint_as_float(r[c * ACC + 2 * i + 1]);
+        if (bias && a0 + 2 * i < p.N) {
+          g += __ldg(bias + a0 + 2 * i);
+          u += __ldg(bias + a0 + 2 * i + 1);
+        }
+        v[i] = mx_swiglu7(g, u) * rw;
+      } else {
+        float z = __uint_as_float(r[c * ACC + i]);
+        if (bias && a0 + i < p.N) z += __ldg(bias + a0 + i);
+        v[i] = z * rw;
+      }
+    }
+    __syncwarp();                                   // the chunk before has left the staging
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (OUT32) w[j] = __float_as_uint(v[4 * k + j]);
+        else w[j] = mg_pack16(v[8 * k + 2 * j], v[8 * k + 2 * j + 1], half);
+      }
+      *reinterpret_cast<uint4*>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+    if (p.y_vec) {
+      constexpr int P16 = PER / 4;                  // outputs of 16 B
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), k = lane & 3;
+        if (q * 32 + row < t.rows && o0 + k * P16 < n_out) {
+          const uint4 w = *reinterpret_cast<const uint4*>(stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4));
+          const int64_t at = (t.row0 + q * 32 + row) * p.y_stride + o0 + k * P16;
+          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + at * (OUT32 ? 4 : 2)) = w;
+        }
+      }
+    } else {
+      // one output a lane (two rows at once in fp32)
+      const int k = OUT32 ? (lane & 15) >> 2 : lane >> 3, b = OUT32 ? (lane & 3) * 4 : (lane & 7) * 2;
+      const int col = o0 + (OUT32 ? (lane & 15) : lane);
+      for (int i = 0; i < (OUT32 ? 16 : 32); ++i) {
+        const int row = OUT32 ? 2 * i + (lane >> 4) : i;
+        if (q * 32 + row >= t.rows || col >= n_out) continue;
+        const uint8_t* src = stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4) + b;
+        const int64_t at = (t.row0 + q * 32 + row) * p.y_stride + col;
+        if constexpr (OUT32) static_cast<uint32_t*>(p.y)[at] = *reinterpret_cast<const uint32_t*>(src);
+        else static_cast<uint16_t*>(p.y)[at] = *reinterpret_cast<const uint16_t*>(src);
+      }
+    }
+  }
+}
+
+// Epilogue of one weight row a thread x up to 32 token columns.
+template <int NC>
+__device__ __forceinline__ void mg_flat_columns(const MgParams& p, const MgTile& t, const uint32_t (&r)[NC], int j0,
+                                                int n, float b) {
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    if (j0 + j >= t.rows) break;
+    const int64_t row = t.row0 + j0 + j;
+    const float rw = p.row_weights ? __ldg(p.row_weights + row) : 1.f;
+    const float z = __uint_as_float(r[j]) + b;
+    if (p.act) {
+      const float u = __shfl_xor_sync(0xffffffffu, z, 1);
+      if (!(n & 1) && n < p.N) mg_store(p.y, p.y_dtype, row * p.y_stride + n / 2, mx_swiglu7(z, u) * rw);
+    } else if (n < p.N) {
+      mg_store(p.y, p.y_dtype, row * p.y_stride + n, z * rw);
+    }
+  }
+}
+
+// tmT: token rows [R, cols_p/2], box 128 B x SLOT; tmW: weight rows [n * N, cols_p/2], box 128 B x WROWS.
+// SPLIT (flat only): a cluster of CTAs shares one work item along K; their partial
+// accumulators meet in distributed shared memory and are summed in the order of the ranks.
+template <bool FLAT, int BN, bool SPLIT, bool OUT32, bool SWIGLU>
+__global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
+                   const MgParams p) {
+  pdl_wait();
+  pdl_trigger();
+  using S = MgShape<FLAT, BN>;
+  constexpr int STAGES = S::STAGES, EPW = S::EPW, COPIER = 2 + EPW, NACC = S::NACC;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + STAGES * MG_A_BYTES;
+  uint8_t* sSFA = sB + STAGES * S::B_BYTES;
+  uint8_t* sSFB = sSFA + STAGES * MG_SFA_BYTES;
+  uint8_t* sSTG = sSFB + STAGES * S::SFB_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + S::STG);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* sff_bar = empty_bar + STAGES;      // the stage's scales are in TMEM
+  uint64_t* tfull_bar = sff_bar + STAGES;      // [NACC]
+  uint64_t* tempty_bar = tfull_bar + NACC;     // [NACC]
+  uint64_t* drain_bar = tempty_bar + NACC;     // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
+  static_assert((3 * STAGES + 2 * NACC + 2) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+      mbar_init(smem_u32(&sff_bar[s]), 1);
+    }
+    for (int a = 0; a < NACC; ++a) {
+      mbar_init(smem_u32(&tfull_bar[a]), 1);
+      mbar_init(smem_u32(&tempty_bar[a]), EPW);
+    }
+    mbar_init(smem_u32(&drain_bar[0]), 1);
+    mbar_init(smem_u32(&drain_bar[1]), 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmT);
+    tma_prefetch_desc(&tmW);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), MG_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int n_tiles = p.n_tiles ? min(*p.n_tiles, p.max_tiles) : p.max_tiles;
+  const int total = n_tiles * p.n_wt;
+  const int n_kblk = (int)((p.katoms + 1) / 2);
+  int t0 = blockIdx.x, step = gridDim.x, kb0 = 0, kb1 = n_kblk, rank = 0, csize = 1;
+  if constexpr (SPLIT) {
+    rank = (int)cluster_ctarank();
+    asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(csize));
+    t0 = blockIdx.x / csize;
+    step = 1 << 30;                            // one item per cluster
+    kb0 = n_kblk * rank / csize;
+    kb1 = n_kblk * (rank + 1) / csize;
+  }
+  const uint64_t timeout = p.timeout_ns ? p.timeout_ns : 2000000000ull;
+
+  if (warp == 0) {
+    // ───────── producer ─────────
+    int stage = 0;
+    uint32_t phase = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    const uint32_t wblk = (uint32_t)((p.N + 127) / 128);
+    for (int64_t t = t0; ok && t < total; t += step) {
+      const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
+      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const int wrow = tile.e * p.N + wt * S::WROWS;
+      const uint32_t wb = wt * (S::WROWS / 128);
+      const uint8_t* sf_t = p.sf_tok + (uint64_t)tile.slot * p.katoms * 512;
+      const uint8_t* sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wb) * p.katoms * 512;
+      const bool second = S::WROWS == 256 && wb + 1 < wblk;       // the weight tile's second atom block exists
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t fb = smem_u32(&full_bar[stage]);
+          const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;  // atoms of this stage
+          mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * (2 + (second ? 1 : 0)));
+          const uint32_t a = smem_u32(sA + stage * MG_A_BYTES), b = smem_u32(sB + stage * S::B_BYTES);
+          const uint32_t sa = smem_u32(sSFA + stage * MG_SFA_BYTES), sb = smem_u32(sSFB + stage * S::SFB_BYTES);
+          tma_load_2d(FLAT ? b : a, &tmT, fb, kb * (MG_BK / 2), (int)tile.row0);
+          tma_load_2d(FLAT ? a : b, &tmW, fb, kb * (MG_BK / 2), wrow);
+          bulk_load(FLAT ? sb : sa, sf_t + kb * 1024, sfn, fb);
+          bulk_load(FLAT ? sa : sb, sf_w + kb * 1024, sfn, fb);
+          if (second) bulk_load(sb + MG_SFA_BYTES, sf_w + (uint64_t)p.katoms * 512 + kb * 1024, sfn, fb);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    // every copy lands before the CTA can exit (returns at once unless a consumer gave up)
+    for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+      mbar_wait(smem_u32(&full_bar[i % STAGES]), (uint32_t)((i / STAGES) & 1), nullptr, 0, MHMOE_DRAIN_NS);
+  } else if (warp == 1) {
+    // ───────── MMA issuer ─────────
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    constexpr uint32_t idesc[2] = {idesc_mxf4(MG_BM, BN, 0), idesc_mxf4(MG_BM, BN, 2)};
+    for (int64_t t = t0; t < total; t += step) {
+      if (!mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+      tc_fence_after();
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+        if (!mbar_wait(smem_u32(&sff_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
+          const uint32_t a_s = smem_u32(sA + stage * MG_A_BYTES);
+          const uint32_t b_s = smem_u32(sB + stage * S::B_BYTES);
+          const int nj = (int)min(4u, 2 * (p.katoms - 2 * kb));    // 64-column steps of this stage
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j < nj)
+              mma_mxf4(tmem_base + acc * BN, sdesc_kmajor_sw128(a_s + j * 32), sdesc_kmajor_sw128(b_s + j * 32),
+                       idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 4 * S::NBLK,
+                       (kb > kb0 || j > 0) ? 1u : 0u);
+          }
+          tc_commit(smem_u32(&empty_bar[stage]));
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+      if (lane == 0) tc_commit(smem_u32(&tfull_bar[acc]));
+      __syncwarp();
+      if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
+    }
+  } else if (warp == COPIER) {
+    // ───────── scale copier ─────────
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int64_t t = t0; t < total; t += step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
+          const uint32_t sa = smem_u32(sSFA + stage * MG_SFA_BYTES), sb = smem_u32(sSFB + stage * S::SFB_BYTES);
+#pragma unroll
+          for (int a = 0; a < 2; ++a) {
+            if (2 * kb + a < (int)p.katoms) {
+              tc_cp_32x128b_warpx4(tsfa + a * 4, sdesc_sf_chunk(sa + a * 512));
+#pragma unroll
+              for (int b = 0; b < S::NBLK; ++b)
+                tc_cp_32x128b_warpx4(tsfb + (a * S::NBLK + b) * 4, sdesc_sf_chunk(sb + b * MG_SFA_BYTES + a * 512));
+            }
+          }
+          tc_commit(smem_u32(&sff_bar[stage]));
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+  } else {
+    // ───────── epilogue ─────────
+    const int q = warp & 3;                    // TMEM lane quarter of this warp
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int64_t t = t0; t < total; t += step) {
+      const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
+      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      if (!mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
+      tc_fence_after();
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+      if constexpr (!FLAT) {
+        const int half = (warp - 2) >> 2;      // accumulator columns [128 * half, +128)
+        uint32_t r[128];
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) MHMOE_TMEM_LD_32x32b_X32(taddr + half * 128 + c, (r + c));
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+        if (q * 32 < tile.rows)
+          mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * 256 + half * 128, q, lane, sSTG + (warp - 2) * MG_STG_BYTES);
+      } else {
+        const int n = wt * 128 + q * 32 + lane;
+        const float b = p.bias && n < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n) : 0.f;
+        constexpr int NC = BN < 32 ? BN : 32;
+        for (int j0 = 0; j0 < BN && j0 < tile.rows; j0 += NC) {
+          uint32_t r[NC];
+          if constexpr (NC == 16) MHMOE_TMEM_LD_32x32b_X16(taddr + j0, r);
+          else MHMOE_TMEM_LD_32x32b_X32(taddr + j0, r);
+          tmem_wait_ld();
+          if constexpr (SPLIT) {
+            // partial sums [token][weight row] over the stages' memory, all of it consumed by now
+            float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+            for (int j = 0; j < NC; ++j) red[(j0 + j) * 128 + q * 32 + lane] = __uint_as_float(r[j]);
+          } else {
+            mg_flat_columns<NC>(p, tile, r, j0, n, b);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
+      }
+      if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
+    }
+  }
+done:
+  // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
+  if (warp == 1 && lane == 0) {
+    tc_commit(smem_u32(&drain_bar[0]));
+    mbar_wait(smem_u32(&drain_bar[0]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+  }
+  if (warp == COPIER && lane == 0) {
+    tc_commit(smem_u32(&drain_bar[1]));
+    mbar_wait(smem_u32(&drain_bar[1]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, MG_TMEM_COLS);
+  }
+  if constexpr (SPLIT) {
+    cluster_sync();
+    if (t0 < total) {
+      const int tt = t0 / p.n_wt, wt = t0 % p.n_wt;
+      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const uint32_t red = smem_u32(smem);
+      uint32_t peer[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) peer[c] = mapa_shared(red, (uint32_t)min(c, csize - 1));
+      auto sum = [&](int at) {                 // partial sums of one output in the order of the ranks
+        float z = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          float v = 0.f;
+          if (c < csize)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer[c] + at * 4) : "memory");
+          z += v;
+        }
+        return z;
+      };
+      const float* bias = p.bias ? p.bias + (int64_t)tile.e * p.N : nullptr;
+      const int per_row = p.act ? 64 : 128;    // outputs of a token in this tile
+      for (int i = threadIdx.x + blockDim.x * rank; i < tile.rows * per_row; i += blockDim.x * csize) {
+        const int j = i / per_row, c = i % per_row;
+        const int64_t row = tile.row0 + j;
+        const float rw = p.row_weights ? __ldg(p.row_weights + row) : 1.f;
+        if (p.act) {
+          const int n = wt * 128 + 2 * c;
+          if (n < p.N) {
+            float g = sum(j * 128 + 2 * c), u = sum(j * 128 + 2 * c + 1);
+            if (bias) {
+              g += __ldg(bias + n);
+              u += __ldg(bias + n + 1);
+            }
+            mg_store(p.y, p.y_dtype, row * p.y_stride + n / 2, mx_swiglu7(g, u) * rw);
+          }
+        } else {
+          const int n = wt * 128 + c;
+          if (n < p.N) {
+            float z = sum(j * 128 + c);
+            if (bias) z += __ldg(bias + n);
+            mg_store(p.y, p.y_dtype, row * p.y_stride + n, z * rw);
+          }
+        }
+      }
+    }
+    cluster_sync();                            // no CTA leaves while others read its memory
+  }
+}
+
+// ───────────────────────────── expert rows ─────────────────────────────
+
+__device__ __forceinline__ int64_t clip(int64_t v, int64_t hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
+
+struct MgGroup {
+  int64_t x_stride, x_rows, R;
+  uint32_t cols, katoms;
+  bool ceil, vec;
+  const int64_t* offsets;
+  int n, slot_rows, max_tiles;
+  const int32_t* gather;
+  uint8_t* data;              // [R, katoms * 64]
+  uint8_t* sf;                // slots of katoms atoms
+  int4* tiles;
+  int* n_tiles;
+  uint8_t* y;                 // rows without an expert are cleared
+  int64_t y_row_bytes, y_pitch;
   bool zero_tail;
   int* status;
 };
 
-__device__ __forceinline__ int64_t clip(int64_t v, int64_t hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
-
-// 64 x 64 outputs per CTA, 256 threads of 4 x 4, one scale block of K at a time.
+// Block 0 lists the token tiles; every other warp quantises one sorted row.  Expert e's tiles
+// take the scale slots offsets[e] / slot_rows + e + 0, 1, ...: the sum of the rounded-up tile
+// counts before e is at most that, so no prefix sum has to come first.
 template <int DT>
-__global__ void __launch_bounds__(256) mx_product_simple_kernel(const SimpleArgs p, typename MxType<DT>::T* y) {
+__global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>::T* __restrict__ x, const MgGroup p) {
   pdl_wait();
   pdl_trigger();
-  __shared__ float xs[SG_BK][SG_BM + 1], ws[SG_BK][SG_BN + 1];
-  const int n0 = blockIdx.x * SG_BN;
-  const int64_t t = blockIdx.y;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x == 0) {
+    __shared__ int wsum[8];
+    int base = 0;
+    bool bad = false;
+    for (int e0 = 0; e0 < p.n; e0 += 256) {
+      const int e = e0 + threadIdx.x;
+      int64_t a = 0;
+      int rows = 0;
+      if (e < p.n) {
+        const int64_t lo = p.offsets[e], hi = p.offsets[e + 1];
+        bad |= lo < 0 || lo > p.R || hi < lo || hi > p.R;
+        a = clip(lo, p.R);
+        rows = (int)max((int64_t)0, clip(hi, p.R) - a);
+      }
+      const int cnt = (rows + p.slot_rows - 1) / p.slot_rows;
+      int inc = cnt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) wsum[warp] = inc;
+      __syncthreads();
+      int before = 0, all = 0;
+      for (int w = 0; w < 8; ++w) {
+        before += w < warp ? wsum[w] : 0;
+        all += wsum[w];
+      }
+      const int at = base + before + inc - cnt;
+      const int slot0 = (int)(a / p.slot_rows) + e;
+      for (int j = 0; j < cnt && at + j < p.max_tiles; ++j)
+        p.tiles[at + j] = make_int4(e, (int)a + j * p.slot_rows, min(p.slot_rows, rows - j * p.slot_rows), slot0 + j);
+      base += all;
+      __syncthreads();
+    }
+    if (threadIdx.x == 0) *p.n_tiles = min(base, p.max_tiles);
+    if (bad) record_error(p.status, MHMOE_ERR_ARGS);
+    return;
+  }
+  const int64_t r = (int64_t)(blockIdx.x - 1) * 8 + warp;
+  if (r >= p.R) return;
+  // the last expert whose first row is at or before r
   int e = 0;
-  int64_t row0 = t * SG_BM, row1 = p.R;
-  if (p.offsets) {
-    int lo = 0, hi = p.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (clip(p.offsets[mid], p.R) / SG_BM + mid <= t) lo = mid;
-      else hi = mid - 1;
+  int64_t a = 0;
+  bool none = clip(p.offsets[0], p.R) > r || clip(p.offsets[p.n], p.R) <= r;
+  if (!none) {
+    int len = p.n;
+    while (len > 1) {
+      const int step = (len + 31) / 32, i = e + lane * step;
+      const bool le = lane * step < len && clip(p.offsets[i], p.R) <= r;
+      const int k = max(__popc(__ballot_sync(0xffffffffu, le)), 1) - 1;
+      e += k * step;
+      len = min(step, len - k * step);
     }
-    e = lo;
-    const int64_t a = clip(p.offsets[e], p.R);
-    row1 = clip(p.offsets[e + 1], p.R);
-    row0 = a + (t - (a / SG_BM + e)) * SG_BM;
-    if (t == 0 && blockIdx.x == 0) {
-      for (int i = threadIdx.x; i <= p.n; i += 256) {
-        const int64_t o = p.offsets[i];
-        if (o < 0 || o > p.R || (i > 0 && o < p.offsets[i - 1])) record_error(p.status, MHMOE_ERR_ARGS);
-      }
-    }
-    if (p.zero_tail && t == 0) {
-      const int cols = p.act ? p.N / 2 : p.N, c0 = p.act ? n0 / 2 : n0, nc = min(p.act ? SG_BN / 2 : SG_BN, cols - c0);
-      for (int64_t r = clip(p.offsets[p.n], p.R); r < p.R; ++r)
-        for (int c = threadIdx.x; c < nc; c += 256) mx_store(y + r * p.y_stride + c0 + c, 0.f);
-    }
+    a = clip(p.offsets[e], p.R);
+    none = a > r;                                // only with offsets that decrease
   }
-  if (row0 >= row1) return;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  float acc[4][4] = {};
-  for (uint32_t kb = 0; kb < p.katoms * 4; ++kb) {
-    for (int i = threadIdx.x; i < 2 * 64 * 4; i += 256) {
-      const int which = i >> 8, r = (i >> 2) & 63, q = i & 3;
-      float v[8] = {};
-      if (which == 0) {
-        const int64_t row = row0 + r;
-        int64_t src = row;
-        bool ok = row < row1;
-        if (ok && p.gather) {
-          src = p.gather[row];
-          ok = src >= 0 && src < p.x_rows;
-          if (!ok && kb == 0) record_error(p.status, MHMOE_ERR_ARGS);
-        }
-        if (ok) {
-          mx_decode8(*reinterpret_cast<const uint32_t*>(p.xq + src * p.katoms * 64 + kb * 16 + q * 4), v);
-          const float s = mx_scale_value(p.xsf[mx_sf_offset(src, kb, p.katoms)]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= s;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) xs[q * 8 + j][r] = v[j];
-      } else {
-        const int64_t row = n0 + r;
-        if (row < p.N) {
-          const uint64_t base = (uint64_t)e * ((p.N + 127) / 128) * p.katoms * 512;
-          mx_decode8(*reinterpret_cast<const uint32_t*>(p.w + ((int64_t)e * p.N + row) * p.katoms * 64 + kb * 16 + q * 4), v);
-          const float s = mx_scale_value(p.wsf[base + mx_sf_offset(row, kb, p.katoms)]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] *= s;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ws[q * 8 + j][r] = v[j];
-      }
+  if (none) {
+    if (p.zero_tail) {
+      uint8_t* o = p.y + r * p.y_pitch;          // elements of 2 or 4 bytes
+      for (int64_t i = lane * 2; i < p.y_row_bytes; i += 64) *reinterpret_cast<uint16_t*>(o + i) = 0;
     }
-    __syncthreads();
+    return;
+  }
+  const int m = (int)(r - a) % p.slot_rows;
+  const int64_t slot = a / p.slot_rows + e + (r - a) / p.slot_rows;
+  int64_t src = p.gather ? p.gather[r] : r;
+  const bool ok = src >= 0 && src < p.x_rows;
+  if (!ok && lane == 0) record_error(p.status, MHMOE_ERR_ARGS);
+  const typename MxType<DT>::T* xr = x + (ok ? src : 0) * p.x_stride;
+  uint8_t* d = p.data + r * (int64_t)p.katoms * 64;
+  uint8_t* s = p.sf + (uint64_t)slot * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
 #pragma unroll 4
-    for (int k = 0; k < SG_BK; ++k) {
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = xs[k][ty * 4 + i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = ws[k][tx * 4 + j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(a[i], b[j], acc[i][j]);
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t row = row0 + ty * 4 + i;
-    if (row >= row1) break;
-    const float rw = p.row_weights ? p.row_weights[row] : 1.f;
-    float o[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = n0 + tx * 4 + j;
-      o[j] = acc[i][j] + (p.bias && c < p.N ? p.bias[(int64_t)e * p.N + c] : 0.f);
-    }
-    if (p.act) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int c = (n0 + tx * 4) / 2 + j;
-        if (2 * c < p.N) mx_store(y + row * p.y_stride + c, mx_swiglu7(o[2 * j], o[2 * j + 1]) * rw);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = n0 + tx * 4 + j;
-        if (c < p.N) mx_store(y + row * p.y_stride + c, o[j] * rw);
-      }
+  for (uint32_t c0 = lane * 8; c0 < ((p.katoms + 1) & ~1u) * 128; c0 += 256) {
+    float v[8] = {};
+    if (ok && c0 < p.cols) mx_load8(xr + c0, p.vec && c0 + 8 <= p.cols, (int)min(8u, p.cols - c0), v);
+    uint32_t sw;
+    const uint32_t w = mx_quantize8(v, p.ceil, lane & 15, 0xffffffffu, sw);
+    if (c0 < p.katoms * 128) {
+      *reinterpret_cast<uint32_t*>(d + c0 / 2) = w;
+      if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(s + (c0 / 128) * 512) = sw;
     }
   }
+}
+
+// ───────────────────────────── launch ─────────────────────────────
+
+struct MgPlan {
+  bool flat;
+  int bn, slot_rows, split;
+  int64_t tiles, slots;       // token tiles at most; scale slots
+  int n_wt;
+};
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Orientation, tile and split by the sizes alone.
+MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
+  const int sms = num_sms();
+  MgPlan g;
+  const int64_t avg = grouped ? ceil_div(R, n) : R;
+  auto tiles_of = [&](int64_t slot) { return grouped ? R / slot + std::min<int64_t>(n, R) : ceil_div(R, slot); };
+  if (avg <= 64 || (!grouped && R <= 128)) {
+    // a few rows per matrix: one flat tile holds them
+    const int64_t want = grouped ? avg + avg / 2 : avg;
+    g.flat = true;
+    g.bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
+  } else {
+    g.flat = tiles_of(128) * ceil_div(N, 256) < sms;
+    g.bn = g.flat ? 128 : 256;
+  }
+  g.slot_rows = g.flat ? g.bn : 128;
+  g.tiles = tiles_of(g.slot_rows);
+  g.slots = grouped ? R / g.slot_rows + n + 1 : g.tiles;
+  g.n_wt = (int)ceil_div(N, g.flat ? 128 : 256);
+  g.split = 1;
+  const int64_t n_kblk = ceil_div(katoms, 2);
+  while (g.flat && g.split < 8 && g.tiles * g.n_wt * g.split * 2 <= sms && g.split * 2 <= n_kblk) g.split *= 2;
+  return g;
+}
+
+struct MgScratch {
+  size_t data, sf, tiles, count, bytes;
+};
+MgScratch mg_scratch(const MgPlan& g, int64_t R, int64_t katoms, bool grouped) {
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  MgScratch s;
+  s.data = 0;
+  s.sf = up((size_t)R * katoms * 64);
+  s.tiles = s.sf + up((size_t)(grouped ? g.slots : ceil_div(R, 128)) * katoms * 512);
+  s.count = s.tiles + (grouped ? up((size_t)g.tiles * sizeof(int4)) : 0);
+  s.bytes = s.count + (grouped ? 256 : 0);
+  return s;
+}
+
+template <bool FLAT, int BN, bool SPLIT, bool OUT32, bool SWIGLU>
+cudaError_t mg_launch(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                      cudaStream_t st) {
+  using S = MgShape<FLAT, BN>;
+  auto kernel = mx_gemm_kernel<FLAT, BN, SPLIT, OUT32, SWIGLU>;
+  static PerDeviceOnce once;
+  const cudaError_t attr = once.run(
+      [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
+  if (attr != cudaSuccess) return attr;
+  const int64_t items = g.tiles * g.n_wt;
+  if constexpr (!SPLIT) {
+    return launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(num_sms(), items)), dim3(S::THREADS), S::SMEM, st, tt, tw,
+                      p);
+  } else {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * g.split));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attrs[2];
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = 1;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = (unsigned)g.split;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg.attrs = attrs;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kernel, tt, tw, p);
+  }
+}
+
+template <int BN>
+cudaError_t mg_launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                           cudaStream_t st) {
+  return g.split > 1 ? mg_launch<true, BN, true, false, false>(tt, tw, p, g, st)
+                     : mg_launch<true, BN, false, false, false>(tt, tw, p, g, st);
 }
 
 }  // namespace
 
 size_t mx_product_workspace_bytes(int64_t x_rows, int64_t R, int n, int N, int cols, bool grouped) {
   const int64_t katoms = mx_padded_cols(cols) / 128;
-  return (size_t)((x_rows * katoms * 64 + 255) / 256 * 256 + (x_rows + 127) / 128 * katoms * 512);
+  if (R == 0) return 0;
+  return mg_scratch(mg_plan(R, n, N, katoms, grouped), R, katoms, grouped).bytes;
 }
 
 int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t* cerr) {
   const int64_t katoms = mx_padded_cols(p.cols) / 128;
-  const uint8_t* xq = p.xq;
-  const uint8_t* xsf = p.xsf;
-  if (!xq) {
-    uint8_t* d = static_cast<uint8_t*>(workspace);
-    uint8_t* s = d + (p.x_rows * katoms * 64 + 255) / 256 * 256;
-    *cerr = launch_mx_quantize(p.x, p.x_dtype, 0, p.x_stride, 1, p.x_rows, p.cols, p.ceil, d, s, st);
-    if (*cerr != cudaSuccess) return MHMOE_ERR_LAUNCH;
-    xq = d;
-    xsf = s;
+  const bool grouped = p.offsets != nullptr;
+  const MgPlan g = mg_plan(p.R, p.n, p.N, katoms, grouped);
+  if (g.tiles * g.n_wt >= (int64_t)1 << 30) return MHMOE_ERR_CAPACITY;
+  const MgScratch ws = mg_scratch(g, p.R, katoms, grouped);
+  uint8_t* base = static_cast<uint8_t*>(workspace);
+  const int64_t y_esz = p.y_dtype == DT_F32 ? 4 : 2, n_out = p.act ? p.N / 2 : p.N;
+  const uint8_t* data = p.xq;
+  MgParams a{};
+  a.sf_tok = p.xsf;
+  if (grouped) {
+    const int64_t esz = p.x_dtype == DT_F32 ? 4 : 2;
+    MgGroup q{};
+    q.x_stride = p.x_stride;
+    q.x_rows = p.x_rows;
+    q.R = p.R;
+    q.cols = (uint32_t)p.cols;
+    q.katoms = (uint32_t)katoms;
+    q.ceil = p.ceil;
+    q.vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.x_stride * esz % 16 == 0;
+    q.offsets = p.offsets;
+    q.n = p.n;
+    q.slot_rows = g.slot_rows;
+    q.max_tiles = (int)g.tiles;
+    q.gather = p.gather_ids;
+    q.data = base + ws.data;
+    q.sf = base + ws.sf;
+    q.tiles = reinterpret_cast<int4*>(base + ws.tiles);
+    q.n_tiles = reinterpret_cast<int*>(base + ws.count);
+    q.y = static_cast<uint8_t*>(p.y);
+    q.y_row_bytes = n_out * y_esz;
+    q.y_pitch = p.y_stride * y_esz;
+    q.zero_tail = p.zero_tail;
+    q.status = p.status;
+    const unsigned grid = (unsigned)(1 + ceil_div(p.R, 8));
+    if (p.x_dtype == DT_F32)
+      *cerr = launch_pdl(mx_group_kernel<DT_F32>, dim3(grid), dim3(256), 0, st, static_cast<const float*>(p.x), q);
+    else if (p.x_dtype == DT_BF16)
+      *cerr = launch_pdl(mx_group_kernel<DT_BF16>, dim3(grid), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(p.x), q);
+    else
+      *cerr = launch_pdl(mx_group_kernel<DT_F16>, dim3(grid), dim3(256), 0, st, static_cast<const __half*>(p.x), q);
+    data = q.data;
+    a.sf_tok = q.sf;
+    a.tiles = q.tiles;
+    a.n_tiles = q.n_tiles;
+  } else if (!p.xq) {
+    *cerr = launch_mx_quantize(p.x, p.x_dtype, 0, p.x_stride, 1, p.R, p.cols, p.ceil, base + ws.data, base + ws.sf, st);
+    data = base + ws.data;
+    a.sf_tok = base + ws.sf;
   }
-  SimpleArgs a{xq, xsf, p.w_data, p.w_sf, p.n, p.N, (uint32_t)katoms, p.offsets, p.gather_ids, p.R, p.x_rows,
-               p.row_weights, p.bias, p.act, p.y_stride, p.zero_tail, p.status};
-  const int64_t slots = p.offsets ? p.R / SG_BM + p.n : (p.R + SG_BM - 1) / SG_BM;
-  const dim3 grid((p.N + SG_BN - 1) / SG_BN, (unsigned)slots);
-  if (p.y_dtype == DT_F32)
-    *cerr = launch_pdl(mx_product_simple_kernel<DT_F32>, grid, dim3(256), 0, st, a, static_cast<float*>(p.y));
-  else if (p.y_dtype == DT_BF16)
-    *cerr = launch_pdl(mx_product_simple_kernel<DT_BF16>, grid, dim3(256), 0, st, a, static_cast<__nv_bfloat16*>(p.y));
-  else
-    *cerr = launch_pdl(mx_product_simple_kernel<DT_F16>, grid, dim3(256), 0, st, a, static_cast<__half*>(p.y));
+  if (*cerr != cudaSuccess) return MHMOE_ERR_LAUNCH;
+  a.sf_w = p.w_sf;
+  a.max_tiles = (int)g.tiles;
+  a.R = p.R;
+  a.N = p.N;
+  a.n_wt = g.n_wt;
+  a.katoms = (uint32_t)katoms;
+  a.row_weights = p.row_weights;
+  a.bias = p.bias;
+  a.act = p.act;
+  a.y = p.y;
+  a.y_dtype = p.y_dtype;
+  a.y_stride = p.y_stride;
+  a.y_vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride * y_esz % 16 == 0 && n_out * y_esz % 16 == 0;
+  a.status = p.status;
+  a.timeout_ns = p.timeout_ns;
+  CUtensorMap tt, tw;
+  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)g.slot_rows) != cudaSuccess ||
+      encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, g.flat ? 128 : 256) != cudaSuccess)
+    return MHMOE_ERR_DRIVER;
+  if (g.flat) {
+    *cerr = g.bn == 16   ? mg_launch_flat<16>(tt, tw, a, g, st)
+            : g.bn == 32 ? mg_launch_flat<32>(tt, tw, a, g, st)
+            : g.bn == 64 ? mg_launch_flat<64>(tt, tw, a, g, st)
+                         : mg_launch_flat<128>(tt, tw, a, g, st);
+  } else if (p.y_dtype == DT_F32) {
+    *cerr = p.act ? mg_launch<false, 256, false, true, true>(tt, tw, a, g, st)
+                  : mg_launch<false, 256, false, true, false>(tt, tw, a, g, st);
+  } else {
+    *cerr = p.act ? mg_launch<false, 256, false, false, true>(tt, tw, a, g, st)
+                  : mg_launch<false, 256, false, false, false>(tt, tw, a, g, st);
+  }
   return *cerr == cudaSuccess ? MHMOE_OK : MHMOE_ERR_LAUNCH;
 }
 
