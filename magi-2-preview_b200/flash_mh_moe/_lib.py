@@ -128,6 +128,23 @@ def stream_ptr(device: torch.device | None = None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def launch(name: str, device: torch.device, *args) -> None:
+    """Call entry point ``name`` with ``args`` and the current stream of ``device`` (last argument),
+    with that device current, and raise on an error status.  The short path of the operators
+    whose GPU time is a few microseconds: no context manager, no stream object."""
+    fn = getattr(_lib or lib(), name)
+    idx = device.index
+    cur = torch._C._cuda_getDevice()
+    stream = torch._C._cuda_getCurrentRawStream(idx)
+    if cur == idx:
+        rc = fn(*args, stream)
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, stream)
+    if rc != MHMOE_OK:
+        check(rc, name.removeprefix("mhmoe_"))
+
+
 def require_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:

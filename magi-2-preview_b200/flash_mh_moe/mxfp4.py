@@ -18,6 +18,7 @@ they have no backward pass, and refuse activations that need one.
 """
 from __future__ import annotations
 
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -90,6 +91,16 @@ class MXFP4Matrix:
         return (d, s) if self.batched else (d[0], s[0])
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(x_rows: int, R: int, n: int, N: int, cols: int, grouped: int, device: int) -> int:
+    with torch.cuda.device(device):
+        return max(1, _lib.lib().mhmoe_mxfp4_workspace_bytes(x_rows, R, n, N, cols, grouped))
+
+
+def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    return t if t.dtype == dtype and t.is_contiguous() else t.detach().to(dtype).contiguous()
+
+
 def _check_rounding(scale_rounding: str) -> int:
     if scale_rounding not in _ROUNDING:
         raise ValueError(f"scale_rounding must be 'floor' or 'ceil', got {scale_rounding!r}")
@@ -118,22 +129,22 @@ def mxfp4_quantize(x: torch.Tensor, scale_rounding: str = "floor") -> MXFP4Matri
     that holds NaN or an infinity becomes NaN."""
     rounding = _check_rounding(scale_rounding)
     _check_float(x, "x")
-    if x.dim() not in (2, 3) or x.shape[-1] < 1:
-        raise ValueError(f"mxfp4_quantize takes [rows, cols] or [n, rows, cols], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) not in (2, 3) or shape[-1] < 1:
+        raise ValueError(f"mxfp4_quantize takes [rows, cols] or [n, rows, cols], got {tuple(shape)}")
     _lib.require_cuda(x)
-    x = x.detach()
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
-        x = x.contiguous()
-    x3 = x if x.dim() == 3 else x[None]
-    n, rows, cols = x3.shape
+    rows, cols = shape[-2:]
+    if cols > 1 and x.stride(-1) != 1:
+        x = x.detach().contiguous()
+    batched = len(shape) == 3
+    n, sn = (shape[0], x.stride(0)) if batched else (1, 0)
     dev = x.device
-    data = torch.empty(n, rows, _atoms(cols) * 64, dtype=torch.uint8, device=dev)
-    sf = torch.empty(n, (rows + 127) // 128 * _atoms(cols) * 512, dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().mhmoe_mxfp4_quantize(
-            x3.data_ptr(), _lib.DTYPES[x.dtype], x3.stride(0), x3.stride(1), n, rows, cols, rounding, data.data_ptr(),
-            sf.data_ptr(), _lib.stream_ptr(dev)), "mxfp4_quantize")
-    return MXFP4Matrix(data, sf, rows, cols, n, x.dim() == 3)
+    ka = _atoms(cols)
+    data = torch.empty((n, rows, ka * 64), dtype=torch.uint8, device=dev)
+    sf = torch.empty((n, (rows + 127) // 128 * ka * 512), dtype=torch.uint8, device=dev)
+    _lib.launch("mhmoe_mxfp4_quantize", dev, x.data_ptr(), _lib.DTYPES[x.dtype], sn, x.stride(-2), n, rows, cols, rounding,
+                data.data_ptr(), sf.data_ptr())
+    return MXFP4Matrix(data, sf, rows, cols, n, batched)
 
 
 def mxfp4_dequantize(m: MXFP4Matrix, dtype: torch.dtype = torch.float32) -> torch.Tensor:
@@ -144,10 +155,8 @@ def mxfp4_dequantize(m: MXFP4Matrix, dtype: torch.dtype = torch.float32) -> torc
         raise ValueError(f"dtype must be fp32, bf16 or fp16, got {dtype}")
     dev = m.device
     out = torch.empty(m.shape, dtype=dtype, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.lib().mhmoe_mxfp4_dequantize(
-            m.data.data_ptr(), m.sf.data_ptr(), m.num_matrices, m.rows, m.cols, _lib.DTYPES[dtype], out.data_ptr(),
-            _lib.stream_ptr(dev)), "mxfp4_dequantize")
+    _lib.launch("mhmoe_mxfp4_dequantize", dev, m.data.data_ptr(), m.sf.data_ptr(), m.num_matrices, m.rows, m.cols,
+                _lib.DTYPES[dtype], out.data_ptr())
     return out
 
 
@@ -165,7 +174,8 @@ def _product_args(x, bias, activation, n, N, out_dtype, what, row_weights=None):
             raise ValueError(f"bias must hold {n} x {N} values, got {tuple(bias.shape)}")
         if bias.device != x.device:
             raise ValueError(f"bias is on {bias.device}, the activations on {x.device}")
-        bias = bias.detach().float().contiguous()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().float().contiguous()
     return bias, _ACTIVATION[activation], (N // 2 if activation else N)
 
 
@@ -198,23 +208,20 @@ def mxfp4_linear(x: torch.Tensor | MXFP4Matrix, weight: MXFP4Matrix, bias: torch
     dtype = out_dtype or (torch.bfloat16 if quantized else x.dtype)
     bias, act, n_out = _product_args(ref, bias, activation, 1, N, dtype, "mxfp4_linear")
     dev = ref.device
-    M = 1
-    for v in lead:
-        M *= v
-    y = torch.empty(*lead, n_out, dtype=dtype, device=dev)
-    L = _lib.lib()
-    x2 = ws = None
-    if not quantized:
-        x2 = x.detach().reshape(M, cols)
+    M = x.rows if quantized else (x.numel() // cols if cols else 0)
+    y = torch.empty((*lead, n_out), dtype=dtype, device=dev)
+    x2, xd, xs, ws, xq, xsf = None, 0, 0, None, None, None
+    if quantized:
+        xq, xsf = x.data.data_ptr(), x.sf.data_ptr()
+    else:
+        x2 = x if x.dim() == 2 else x.detach().reshape(M, cols)
         if cols > 1 and x2.stride(1) != 1:
-            x2 = x2.contiguous()
-        ws = torch.empty(max(1, L.mhmoe_mxfp4_workspace_bytes(M, M, 1, N, cols, 0)), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(L.mhmoe_mxfp4_linear(
-            _lib.ptr(x2), 0 if quantized else _lib.DTYPES[x.dtype], 0 if quantized else x2.stride(0),
-            x.data.data_ptr() if quantized else None, x.sf.data_ptr() if quantized else None, M, cols, rounding,
-            weight.data.data_ptr(), weight.sf.data_ptr(), N, _lib.ptr(bias), act, _lib.ptr(ws), y.data_ptr(),
-            _lib.DTYPES[dtype], n_out, _lib.device_status(dev).data_ptr(), 0, _lib.stream_ptr(dev)), "mxfp4_linear")
+            x2 = x2.detach().contiguous()
+        xd, xs = _lib.DTYPES[x.dtype], x2.stride(0)
+        ws = torch.empty(_workspace_bytes(M, M, 1, N, cols, 0, dev.index), dtype=torch.uint8, device=dev)
+    _lib.launch("mhmoe_mxfp4_linear", dev, _lib.ptr(x2), xd, xs, xq, xsf, M, cols, rounding, weight.data.data_ptr(),
+                weight.sf.data_ptr(), N, _lib.ptr(bias), act, _lib.ptr(ws), y.data_ptr(), _lib.DTYPES[dtype], n_out,
+                _lib.device_status(dev).data_ptr(), 0)
     return y
 
 
@@ -263,19 +270,15 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
     if out is not None and (tuple(out.shape) != (R, n_out) or out.dtype != dtype or out.device != dev
                             or (n_out > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < n_out)):
         raise ValueError(f"out must be [{R}, {n_out}] {dtype} on {dev} with unit inner stride")
-    xs = x.detach()
-    if cols > 1 and xs.stride(1) != 1:
-        xs = xs.contiguous()
-    offs = expert_offsets.to(torch.int64).contiguous()
-    gids = None if gather_ids is None else gather_ids.to(torch.int32).contiguous()
-    rw = None if row_weights is None else row_weights.detach().float().contiguous()
-    y = torch.empty(R, n_out, dtype=dtype, device=dev) if out is None else out
-    L = _lib.lib()
-    ws = torch.empty(max(1, L.mhmoe_mxfp4_workspace_bytes(T, R, n, N, cols, 1)), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _lib.check(L.mhmoe_mxfp4_expert_linear(
-            xs.data_ptr(), _lib.DTYPES[x.dtype], xs.stride(0), T, cols, rounding, weight.data.data_ptr(),
-            weight.sf.data_ptr(), n, N, offs.data_ptr(), _lib.ptr(gids), R, _lib.ptr(rw), _lib.ptr(bias), act,
-            ws.data_ptr(), y.data_ptr(), _lib.DTYPES[dtype], max(y.stride(0), n_out), int(out is None),
-            _lib.device_status(dev).data_ptr(), 0, _lib.stream_ptr(dev)), "mxfp4_expert_linear")
+    if cols > 1 and x.stride(1) != 1:
+        x = x.detach().contiguous()
+    offs = _as(expert_offsets, torch.int64)
+    gids = None if gather_ids is None else _as(gather_ids, torch.int32)
+    rw = None if row_weights is None else _as(row_weights, torch.float32)
+    y = torch.empty((R, n_out), dtype=dtype, device=dev) if out is None else out
+    ws = torch.empty(_workspace_bytes(T, R, n, N, cols, 1, dev.index), dtype=torch.uint8, device=dev)
+    _lib.launch("mhmoe_mxfp4_expert_linear", dev, x.data_ptr(), _lib.DTYPES[x.dtype], x.stride(0), T, cols, rounding,
+                weight.data.data_ptr(), weight.sf.data_ptr(), n, N, offs.data_ptr(), _lib.ptr(gids), R, _lib.ptr(rw),
+                _lib.ptr(bias), act, ws.data_ptr(), y.data_ptr(), _lib.DTYPES[dtype], max(y.stride(0), n_out),
+                int(out is None), _lib.device_status(dev).data_ptr(), 0)
     return y

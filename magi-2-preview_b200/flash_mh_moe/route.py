@@ -189,45 +189,60 @@ def route_fused(x_heads: torch.Tensor, planes: torch.Tensor, nsplit: int, num_ex
 
 # ───────────────────────── routing with expert groups, masks and gradients ─────────────────────────
 
+def _route_experts(logits, bias, mask, top_k, cfg, need_saved):
+    """(weights, indices, saved) of validated inputs; cfg = (score id, groups, kept groups, norm, eps, scale)."""
+    H, S, E = logits.shape
+    sh, ss, _ = logits.stride()
+    dev = logits.device
+    weights = torch.empty((H, S, top_k), dtype=torch.float32, device=dev)
+    idx = torch.empty((H, S, top_k), dtype=torch.int64, device=dev)
+    saved = torch.empty((H, S, top_k), dtype=torch.float32, device=dev) if need_saved else None
+    _lib.launch("mhmoe_route_experts", dev, logits.data_ptr(), _lib.DTYPES[logits.dtype], sh, ss,
+                None if bias is None else bias.data_ptr(), None if mask is None else mask.data_ptr(),
+                S if mask is not None and mask.dim() == 2 else 0, H, S, E, top_k, *cfg, weights.data_ptr(),
+                idx.data_ptr(), saved.data_ptr() if need_saved else None)
+    return weights, idx, saved
+
+
+def _route_experts_grad(ctx, grad_w, _grad_idx):
+    if grad_w is None:
+        return (None,) * 5
+    logits, idx, saved = ctx.saved_tensors
+    dtype, E, (score_func, _, _, route_norm, norm_eps, route_scale) = ctx.meta
+    H, S, K = idx.shape
+    g = grad_w if grad_w.dtype == torch.float32 else grad_w.float()
+    gh, gs, gk = g.stride()
+    if gk != 1 and K > 1:
+        g = g.contiguous()
+        gh, gs, _ = g.stride()
+    dev = idx.device
+    out = torch.empty((H, S, E), dtype=dtype, device=dev)
+    ptr, sh, ss = (None, 0, 0) if logits is None else (logits.data_ptr(), logits.stride(0), logits.stride(1))
+    _lib.launch("mhmoe_route_experts_bwd", dev, ptr, _lib.DTYPES[dtype], sh, ss, H, S, E, K, score_func, route_norm,
+                norm_eps, route_scale, g.data_ptr(), gh, gs, idx.data_ptr(), saved.data_ptr(), out.data_ptr())
+    return out, None, None, None, None
+
+
 class _RouteExperts(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, mask, top_k, score_func, groups, keep, route_norm, norm_eps, route_scale):
-        H, S, E = logits.shape
-        dev = logits.device
-        weights = torch.empty(H, S, top_k, dtype=torch.float32, device=dev)
-        idx = torch.empty(H, S, top_k, dtype=torch.int64, device=dev)
-        saved = torch.empty(H, S, top_k, dtype=torch.float32, device=dev) if ctx.needs_input_grad[0] else None
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().mhmoe_route_experts(
-                logits.data_ptr(), _lib.DTYPES[logits.dtype], logits.stride(0), logits.stride(1), _lib.ptr(bias),
-                _lib.ptr(mask), 0 if mask is None else mask.stride(0), H, S, E, top_k, score_func, groups, keep,
-                route_norm, norm_eps, route_scale, weights.data_ptr(), idx.data_ptr(), _lib.ptr(saved),
-                _lib.stream_ptr(dev)), "route_experts")
+    def forward(ctx, logits, bias, mask, top_k, cfg):
+        weights, idx, saved = _route_experts(logits, bias, mask, top_k, cfg, True)
         ctx.mark_non_differentiable(idx)
-        if saved is not None:
-            # sigmoid gradients need the chosen experts' logits only, which `saved` holds
-            ctx.save_for_backward(logits if score_func == 0 else None, idx, saved)
-            ctx.meta = (logits.dtype, E, score_func, route_norm, norm_eps, route_scale)
+        ctx.set_materialize_grads(False)      # no zeros for the indices' gradient
+        # sigmoid gradients need the chosen experts' logits only, which `saved` holds
+        ctx.save_for_backward(logits if cfg[0] == 0 else None, idx, saved)
+        ctx.meta = (logits.dtype, logits.shape[2], cfg)
         return weights, idx
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_w, _grad_idx):
-        logits, idx, saved = ctx.saved_tensors
-        dtype, E, score_func, route_norm, norm_eps, route_scale = ctx.meta
-        H, S, K = idx.shape
-        g = grad_w.float()
-        if K > 1 and g.stride(2) != 1:
-            g = g.contiguous()
-        dev = idx.device
-        out = torch.empty(H, S, E, dtype=dtype, device=dev)
-        with torch.cuda.device(dev):
-            _lib.check(_lib.lib().mhmoe_route_experts_bwd(
-                _lib.ptr(logits), _lib.DTYPES[dtype], 0 if logits is None else logits.stride(0),
-                0 if logits is None else logits.stride(1), H, S, E, K, score_func, route_norm, norm_eps, route_scale,
-                g.data_ptr(), g.stride(0), g.stride(1), idx.data_ptr(), saved.data_ptr(), out.data_ptr(),
-                _lib.stream_ptr(dev)), "route_experts backward")
-        return out, None, None, None, None, None, None, None, None, None
+    def backward(ctx, grad_w, grad_idx):
+        # second derivatives are refused; the guard is only set up where one could be asked for
+        if torch.is_grad_enabled():
+            return _route_experts_grad_once(ctx, grad_w, grad_idx)
+        return _route_experts_grad(ctx, grad_w, grad_idx)
+
+
+_route_experts_grad_once = torch.autograd.function.once_differentiable(_route_experts_grad)
 
 
 def route_experts(
@@ -265,24 +280,29 @@ def route_experts(
     selection and gets no gradient.  E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not
     exceed the experts of ``topk_groups`` groups (``ValueError``).
     """
-    if score_func not in score_func_name2id_map:
+    score = score_func_name2id_map.get(score_func)
+    if score is None:
         raise ValueError(f"Unknown score_func: {score_func}")
     if logits.dim() != 3 or logits.dtype not in _lib.DTYPES:
         raise ValueError(f"logits must be [H, S, E] in fp32, bf16 or fp16, got {tuple(logits.shape)} {logits.dtype}")
+    _lib.require_cuda(logits)
     H, S, E = logits.shape
-    _lib.require_cuda(logits, expert_bias, token_mask)
-    for name, t in (("expert_bias", expert_bias), ("token_mask", token_mask)):
-        if t is not None and t.device != logits.device:
-            raise ValueError(f"{name} is on {t.device}, logits on {logits.device}")
     bias = mask = None
     if expert_bias is not None:
-        if expert_bias.numel() != H * E:
-            raise ValueError(f"expert_bias must hold H*E = {H * E} values, got {tuple(expert_bias.shape)}")
-        bias = expert_bias.detach().reshape(H, E).float().contiguous()
+        if expert_bias.device != logits.device or expert_bias.numel() != H * E:
+            raise ValueError(f"expert_bias must hold H*E = {H * E} values on {logits.device}, got "
+                             f"{tuple(expert_bias.shape)} on {expert_bias.device}")
+        bias = expert_bias if expert_bias.dtype == torch.float32 else expert_bias.detach().float()
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     if token_mask is not None:
-        if token_mask.dtype != torch.bool or tuple(token_mask.shape) not in ((S,), (H, S)):
-            raise ValueError(f"token_mask must be bool [S] or [H, S], got {tuple(token_mask.shape)} {token_mask.dtype}")
-        mask = token_mask.contiguous().view(torch.uint8).expand(H, S)
+        if (token_mask.dtype != torch.bool or tuple(token_mask.shape) not in ((S,), (H, S))
+                or token_mask.device != logits.device):
+            raise ValueError(f"token_mask must be bool [S] or [H, S] on {logits.device}, got "
+                             f"{tuple(token_mask.shape)} {token_mask.dtype} on {token_mask.device}")
+        mask = token_mask if token_mask.is_contiguous() else token_mask.contiguous()
     x = logits if E == 1 or logits.stride(2) == 1 else logits.contiguous()
-    return _RouteExperts.apply(x, bias, mask, int(top_k), score_func_name2id_map[score_func], int(num_groups),
-                               int(topk_groups), int(bool(route_norm)), float(norm_eps), float(route_scale))
+    cfg = (score, int(num_groups), int(topk_groups), int(bool(route_norm)), float(norm_eps), float(route_scale))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _RouteExperts.apply(x, bias, mask, int(top_k), cfg)
+    return _route_experts(x, bias, mask, int(top_k), cfg, False)[:2]
