@@ -12,59 +12,59 @@ namespace mhmoe {
 
 constexpr int MXQ_THREADS = 256;
 
-// A thread holds 8 columns (one 4-B word of codes); 4 neighbours make a block, 16 an atom
-// column of 128 (one 4-B word of scales).  Items are (matrix, row, atom column) with the
-// rows of each matrix counted to a multiple of 128, so that every scale byte is written.
+// Eight threads take one atom column (128 columns of a row), 16 columns each: 8 B of codes a
+// thread, one 4-B word of scales.  Items are (matrix, row, atom column) with the rows of each
+// matrix counted to a multiple of 128, so that every scale byte is written.
 template <int DT>
 __global__ void __launch_bounds__(MXQ_THREADS)
     mx_quantize_kernel(const typename MxType<DT>::T* __restrict__ x, int64_t stride_n, int64_t stride_row,
-                       int64_t rows, int64_t rows_p, uint32_t cols, uint32_t katoms, int64_t items, bool ceil,
+                       uint32_t rows, uint32_t cols, FastDiv katoms, FastDiv rows_p, uint32_t items, bool ceil,
                        bool vec_ok, uint8_t* __restrict__ data, uint8_t* __restrict__ sf) {
   pdl_wait();
   pdl_trigger();
-  const int sub = threadIdx.x & 15;
-  for (int64_t it = (int64_t)blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
-       it += (int64_t)gridDim.x * (MXQ_THREADS / 16)) {
-    const uint32_t ka = (uint32_t)(it % katoms);
-    const int64_t rr = it / katoms;
-    const int64_t b = rr / rows_p, row = rr % rows_p;
-    const uint32_t c0 = ka * 128 + sub * 8;
-    float v[8] = {};
-    const bool live = row < rows;
-    if (live && c0 < cols)
-      mx_load8(x + b * stride_n + row * stride_row + c0, vec_ok && c0 + 8 <= cols, (int)min(8u, cols - c0), v);
-    uint32_t sw;
-    // the 16 lanes of an item stay together: items split warps into halves
-    const uint32_t w = mx_quantize8(v, ceil, sub, 0xffffu << (threadIdx.x & 16), sw);
-    if (live) *reinterpret_cast<uint32_t*>(data + (b * rows + row) * (int64_t)katoms * 64 + ka * 64 + sub * 4) = w;
+  const int sub = threadIdx.x & 7;
+  const uint32_t mask = 0xffu << (threadIdx.x & 24);
+  for (uint32_t it = blockIdx.x * (MXQ_THREADS / 8) + (threadIdx.x >> 3); it < items;
+       it += gridDim.x * (MXQ_THREADS / 8)) {
+    const uint32_t rr = katoms.div(it), ka = it - rr * katoms.d;
+    const uint32_t b = rows_p.div(rr), row = rr - b * rows_p.d;
+    const uint32_t c0 = ka * 128 + sub * 16;
+    MxRaw16<typename MxType<DT>::T> v;
+    const bool live = row < rows && c0 < cols;
+    v.load(x + b * stride_n + row * stride_row + c0, live && vec_ok && c0 + 16 <= cols,
+           live ? (int)min(16u, cols - c0) : 0);
+    uint2 code;
+    const uint32_t sw = mx_quantize16(v, ceil, sub, mask, code);
+    if (row < rows)
+      *reinterpret_cast<uint2*>(data + ((uint64_t)b * rows + row) * katoms.d * 64 + ka * 64 + sub * 8) = code;
     if (sub == 0)
-      *reinterpret_cast<uint32_t*>(sf + (uint64_t)b * (rows_p >> 7) * katoms * 512 + mx_sf_offset(row, ka * 4, katoms)) =
-          sw;
+      *reinterpret_cast<uint32_t*>(sf + (uint64_t)b * (rows_p.d >> 7) * katoms.d * 512 +
+                                   mx_sf_offset(row, ka * 4, katoms.d)) = sw;
   }
 }
 
+// Sixteen threads take one atom column, 8 columns each (a 16-B store in a 2-byte type).
 template <int DT>
 __global__ void __launch_bounds__(MXQ_THREADS)
-    mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ sf, int64_t rows,
-                         int64_t rows_p, uint32_t cols, uint32_t katoms, int64_t items, bool vec_ok,
+    mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ sf, FastDiv rows,
+                         uint32_t rows_p, uint32_t cols, FastDiv katoms, uint32_t items, bool vec_ok,
                          typename MxType<DT>::T* __restrict__ out) {
   pdl_wait();
   pdl_trigger();
   using T = typename MxType<DT>::T;
   const int sub = threadIdx.x & 15;
-  for (int64_t it = (int64_t)blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
-       it += (int64_t)gridDim.x * (MXQ_THREADS / 16)) {
-    const uint32_t ka = (uint32_t)(it % katoms);
-    const int64_t rr = it / katoms;
-    const int64_t b = rr / rows, row = rr % rows;
+  for (uint32_t it = blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
+       it += gridDim.x * (MXQ_THREADS / 16)) {
+    const uint32_t rr = katoms.div(it), ka = it - rr * katoms.d;
+    const uint32_t b = rows.div(rr), row = rr - b * rows.d;
     const uint32_t c0 = ka * 128 + sub * 8;
     if (c0 >= cols) continue;
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(data + rr * (int64_t)katoms * 64 + ka * 64 + sub * 4));
-    const float s = mx_scale_value(__ldg(sf + (uint64_t)b * (rows_p >> 7) * katoms * 512 +
-                                         mx_sf_offset(row, ka * 4 + (sub >> 2), katoms)));
+    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(data + (uint64_t)it * 64 + sub * 4));
+    const float s = mx_scale_value(__ldg(sf + (uint64_t)b * (rows_p >> 7) * katoms.d * 512 +
+                                         mx_sf_offset(row, ka * 4 + (sub >> 2), katoms.d)));
     float v[8];
     mx_decode8(w, v);
-    T* o = out + rr * (int64_t)cols + c0;
+    T* o = out + (uint64_t)rr * cols + c0;
     if (vec_ok && c0 + 8 <= cols) {
       __align__(16) T t[8];
 #pragma unroll
@@ -77,9 +77,9 @@ __global__ void __launch_bounds__(MXQ_THREADS)
   }
 }
 
-static unsigned mx_grid(int64_t items) {
-  const int64_t blocks = (items + MXQ_THREADS / 16 - 1) / (MXQ_THREADS / 16);
-  return (unsigned)std::min<int64_t>(blocks, (int64_t)num_sms() * 64);
+// Blocks of `per_block` items each, at most 16 rounds of 8 resident blocks a SM.
+static unsigned mx_grid(int64_t items, int per_block) {
+  return (unsigned)std::min<int64_t>((items + per_block - 1) / per_block, (int64_t)num_sms() * 128);
 }
 
 cudaError_t launch_mx_quantize(const void* x, int dtype, int64_t stride_n, int64_t stride_row, int64_t n,
@@ -87,12 +87,14 @@ cudaError_t launch_mx_quantize(const void* x, int dtype, int64_t stride_n, int64
   const int64_t rows_p = (rows + 127) / 128 * 128, katoms = mx_padded_cols(cols) / 128;
   const int64_t items = n * rows_p * katoms;
   if (items == 0) return cudaSuccess;
+  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;      // above 2^38 elements
   const int64_t esz = dtype == DT_F32 ? 4 : 2;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && stride_n * esz % 16 == 0 && stride_row * esz % 16 == 0;
-#define MX_Q(DT)                                                                                                  \
-  MHMOE_LAUNCH_PDL(mx_quantize_kernel<DT>, mx_grid(items), MXQ_THREADS, 0, st,                                    \
-                   static_cast<const MxType<DT>::T*>(x), stride_n, stride_row, rows, rows_p, (uint32_t)cols,      \
-                   (uint32_t)katoms, items, ceil, vec, data, sf)
+  const unsigned grid = mx_grid(items, MXQ_THREADS / 8);
+#define MX_Q(DT)                                                                                                 \
+  MHMOE_LAUNCH_PDL(mx_quantize_kernel<DT>, grid, MXQ_THREADS, 0, st, static_cast<const MxType<DT>::T*>(x),       \
+                   stride_n, stride_row, (uint32_t)rows, (uint32_t)cols, FastDiv((uint32_t)katoms),              \
+                   FastDiv((uint32_t)rows_p), (uint32_t)items, ceil, vec, data, sf)
   if (dtype == DT_F32) MX_Q(DT_F32);
   else if (dtype == DT_BF16) MX_Q(DT_BF16);
   else MX_Q(DT_F16);
@@ -105,10 +107,13 @@ cudaError_t launch_mx_dequantize(const uint8_t* data, const uint8_t* sf, int64_t
   const int64_t rows_p = (rows + 127) / 128 * 128, katoms = mx_padded_cols(cols) / 128;
   const int64_t items = n * rows * katoms;
   if (items == 0) return cudaSuccess;
+  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;
   const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && cols * (dtype == DT_F32 ? 4 : 2) % 16 == 0;
-#define MX_D(DT)                                                                                                  \
-  MHMOE_LAUNCH_PDL(mx_dequantize_kernel<DT>, mx_grid(items), MXQ_THREADS, 0, st, data, sf, rows, rows_p,          \
-                   (uint32_t)cols, (uint32_t)katoms, items, vec, static_cast<MxType<DT>::T*>(out))
+  const unsigned grid = mx_grid(items, MXQ_THREADS / 16);
+#define MX_D(DT)                                                                                                 \
+  MHMOE_LAUNCH_PDL(mx_dequantize_kernel<DT>, grid, MXQ_THREADS, 0, st, data, sf, FastDiv((uint32_t)rows),        \
+                   (uint32_t)rows_p, (uint32_t)cols, FastDiv((uint32_t)katoms), (uint32_t)items, vec,            \
+                   static_cast<MxType<DT>::T*>(out))
   if (dtype == DT_F32) MX_D(DT_F32);
   else if (dtype == DT_BF16) MX_D(DT_BF16);
   else MX_D(DT_F16);

@@ -10,6 +10,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kernels.cuh"
 
 namespace mhmoe {
@@ -47,30 +49,68 @@ __device__ __forceinline__ void mx_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void mx_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void mx_store(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Eight consecutive elements as fp32; vec: p is 16-B aligned and all eight exist, otherwise
-// only the first `avail` are read and the rest are zero.
-__device__ __forceinline__ void mx_load8(const float* p, bool vec, int avail, float (&v)[8]) {
-  if (vec) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < avail ? p[i] : 0.f;
-  }
-}
+// Sixteen consecutive elements as raw words (fp32: one a word, else two).  vec: p is 16-B aligned
+// and all sixteen exist; otherwise the first `avail` are read and the rest are zero.
 template <typename T>
-__device__ __forceinline__ void mx_load8(const T* p, bool vec, int avail, float (&v)[8]) {
-  if (vec) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* h = reinterpret_cast<const T*>(&a);
+struct MxRaw16 {
+  static constexpr int WORDS = 16 * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void load(const T* p, bool vec, int avail) {
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = mx_to_f32(h[i]);
-  } else {
+      for (int i = 0; i < WORDS / 4; ++i) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < avail ? mx_to_f32(p[i]) : 0.f;
+      for (int i = 0; i < WORDS; ++i) w[i] = 0;
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < avail) w[i] = __float_as_uint(reinterpret_cast<const float*>(p)[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i < avail) w[i / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+      }
+    }
   }
-}
+  // fp32 bits of the largest magnitude (NaN above infinity): magnitudes order like their bits
+  __device__ __forceinline__ uint32_t amax_bits() const {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) a = max(a, w[i] & 0x7fffffffu);
+      return a;
+    } else {
+      uint32_t a = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) a = __vimax3_u16x2(a, w[i] & 0x7fff7fffu, w[i + 1] & 0x7fff7fffu);
+      a = max(a & 0xffffu, a >> 16);
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) return a << 16;
+      else return __float_as_uint(__half2float(__ushort_as_half((unsigned short)a)));
+    }
+  }
+  __device__ __forceinline__ void values(float (&v)[16]) const {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[i] = __uint_as_float(w[i]);
+      } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+};
 
 // Scale byte of a block whose largest magnitude has the fp32 bits `abits` (sign cleared):
 // floor: 2^floor(log2 amax) / 4, ceil: the smallest power of two s with amax <= 6 s.  The
@@ -92,26 +132,40 @@ __device__ __forceinline__ float mx_scale_value(uint32_t b) {
   return __uint_as_float(b == 255u ? 0x7fc00000u : b << 23);
 }
 
-// Quantise the 8 values of a thread: four neighbouring threads hold a block of 32, sixteen (sub =
-// 0..15, all in `mask`) an atom column of 128.  Returns the packed codes; sw is the atom
-// column's four scale bytes, the same word in all sixteen.
-__device__ __forceinline__ uint32_t mx_quantize8(const float (&v)[8], bool ceil, int sub, uint32_t mask, uint32_t& sw) {
-  uint32_t a = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(v[i]) & 0x7fffffffu);
+// Quantise a thread's 16 elements: two neighbouring threads hold a block of 32, eight (sub = 0..7,
+// all in `mask`) an atom column of 128.  code: the 16 packed values; returns the atom column's
+// four scale bytes, the same word in all eight.
+template <typename T>
+__device__ __forceinline__ uint32_t mx_quantize16(const MxRaw16<T>& x, bool ceil, int sub, uint32_t mask,
+                                                  uint2& code) {
+  uint32_t a = x.amax_bits();
   a = max(a, __shfl_xor_sync(mask, a, 1));
-  a = max(a, __shfl_xor_sync(mask, a, 2));
   const uint32_t s = mx_scale_byte(a, ceil);
-  uint32_t w = 0;
-  if (s != 255u) {
-    const float f = mx_inv_scale(s);
-    w = cvt_e2m1x8(v[0] * f, v[1] * f, v[2] * f, v[3] * f, v[4] * f, v[5] * f, v[6] * f, v[7] * f);
-  }
-  sw = s << (8 * (sub >> 2));
+  const float f = s == 255u ? 0.f : mx_inv_scale(s);
+  float v[16];
+  x.values(v);
+  const uint64_t f2 = f2_pack(f, f);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f2_unpack(f2_mul(f2_pack(v[2 * i], v[2 * i + 1]), f2), v[2 * i], v[2 * i + 1]);
+  code.x = cvt_e2m1x8(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]);
+  code.y = cvt_e2m1x8(v[8], v[9], v[10], v[11], v[12], v[13], v[14], v[15]);
+  if (s == 255u) code = make_uint2(0, 0);
+  uint32_t sw = s << (8 * (sub >> 1));
+  sw |= __shfl_xor_sync(mask, sw, 2);
   sw |= __shfl_xor_sync(mask, sw, 4);
-  sw |= __shfl_xor_sync(mask, sw, 8);
-  return w;
+  return sw;
 }
+
+// Division by a fixed d >= 1 of numbers below 2^31: (mulhi(n, mul) + n) >> shift with
+// 2^shift >= d and mul = floor(2^32 (2^shift - d) / d) + 1 (Granlund and Montgomery 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  explicit FastDiv(uint32_t d_) : d(d_), mul(0), shift(0) {
+    while ((1ull << shift) < d) ++shift;
+    mul = (uint32_t)(((1ull << 32) * ((1ull << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ uint32_t div(uint32_t n) const { return (__umulhi(n, mul) + n) >> shift; }
+};
 
 // Eight E2M1 values of a packed word (nibble i = value i) as fp32.
 __device__ __forceinline__ void mx_decode8(uint32_t w, float (&v)[8]) {

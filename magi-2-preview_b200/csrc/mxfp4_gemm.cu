@@ -579,15 +579,16 @@ __global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>
   const typename MxType<DT>::T* xr = x + (ok ? src : 0) * p.x_stride;
   uint8_t* d = p.data + r * (int64_t)p.katoms * 64;
   uint8_t* s = p.sf + (uint64_t)slot * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
-#pragma unroll 4
-  for (uint32_t c0 = lane * 8; c0 < ((p.katoms + 1) & ~1u) * 128; c0 += 256) {
-    float v[8] = {};
-    if (ok && c0 < p.cols) mx_load8(xr + c0, p.vec && c0 + 8 <= p.cols, (int)min(8u, p.cols - c0), v);
-    uint32_t sw;
-    const uint32_t w = mx_quantize8(v, p.ceil, lane & 15, 0xffffffffu, sw);
+#pragma unroll 2
+  for (uint32_t c0 = lane * 16; c0 < (p.katoms + 3) / 4 * 512; c0 += 512) {
+    MxRaw16<typename MxType<DT>::T> v;
+    const bool live = ok && c0 < p.cols;
+    v.load(xr + c0, live && p.vec && c0 + 16 <= p.cols, live ? (int)min(16u, p.cols - c0) : 0);
+    uint2 code;
+    const uint32_t sw = mx_quantize16(v, p.ceil, lane & 7, 0xffffffffu, code);
     if (c0 < p.katoms * 128) {
-      *reinterpret_cast<uint32_t*>(d + c0 / 2) = w;
-      if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(s + (c0 / 128) * 512) = sw;
+      *reinterpret_cast<uint2*>(d + c0 / 2) = code;
+      if ((lane & 7) == 0) *reinterpret_cast<uint32_t*>(s + (c0 / 128) * 512) = sw;
     }
   }
 }

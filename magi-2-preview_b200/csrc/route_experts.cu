@@ -43,16 +43,44 @@ __device__ __forceinline__ void warp_best(double& v, int& i) {
   }
 }
 
-// Row selection in 64 bits.  key: shared [E], value: shared [E] (score + bias; may alias key
-// when there are no groups).  Masked experts hold -inf, NaN holds -DBL_MAX (below every
-// number, above the masked).  Lane k returns the id of the k-th choice (-1: none left).
-__device__ int select64(double* key, double* value, double* gscore, int E, int K, int G, int keep, int lane) {
-  if (G > 1) {
-    const int per = E / G;
+// A row's selection with 64-bit keys, in shared memory val[E] and gscore[64].  Masked experts hold
+// -inf, NaN holds -DBL_MAX (below every number, above the masked).  Lane k returns the id of the
+// k-th choice (-1: none left).
+template <typename T>
+__device__ __noinline__ int select_row64(const RouteArgs& a, const T* lg, const float* bias, double* val, int lane) {
+  const int E = a.E, G = a.groups;
+  double* gscore = val + E;
+  if (a.score_func == 0) {
+    float m = -INFINITY;
+    bool nan = false;
+    for (int e = lane; e < E; e += 32) {
+      const float x = mx_to_f32(lg[e]);
+      nan |= x != x;
+      m = fmaxf(m, x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+    if (__any_sync(FULL, nan)) m = NAN;
+    double sum = 0;
+    for (int e = lane; e < E; e += 32) sum += exp((double)mx_to_f32(lg[e]) - (double)m);
+    sum = warp_sum(sum);
+    for (int e = lane; e < E; e += 32) val[e] = exp((double)mx_to_f32(lg[e]) - (double)m) / sum;
+  } else {
+    for (int e = lane; e < E; e += 32) val[e] = 1.0 / (1.0 + exp(-(double)mx_to_f32(lg[e])));
+  }
+  for (int e = lane; e < E; e += 32) {
+    const float b = bias ? bias[e] : 0.f;
+    const double v = val[e] + (double)b;
+    val[e] = mx_to_f32(lg[e]) == -INFINITY || b == -INFINITY ? -INFINITY : (v != v ? -DBL_MAX : v);
+  }
+  __syncwarp();
+  unsigned long long kept = ~0ull;
+  const int per = E / G;
+  if (a.keep < G) {
     for (int g = lane; g < G; g += 32) {
       double b1 = -INFINITY, b2 = -INFINITY;
       for (int j = 0; j < per; ++j) {
-        const double v = value[g * per + j];
+        const double v = val[g * per + j];
         if (v > b1) {
           b2 = b1;
           b1 = v;
@@ -64,36 +92,40 @@ __device__ int select64(double* key, double* value, double* gscore, int E, int K
       gscore[g] = b1 == -INFINITY ? -INFINITY : fmax(s, -DBL_MAX);
     }
     __syncwarp();
-    unsigned long long chosen = 0;
-    for (int t = 0; t < keep; ++t) {
+    kept = 0;
+    for (int t = 0; t < a.keep; ++t) {
       double v = 0;
       int i = -1;
       for (int g = lane; g < G; g += 32)
-        if (!(chosen >> g & 1ull) && gscore[g] != -INFINITY && (i < 0 || gscore[g] > v)) {
+        if (!(kept >> g & 1ull) && gscore[g] != -INFINITY && (i < 0 || gscore[g] > v)) {
           v = gscore[g];
           i = g;
         }
       warp_best(v, i);
       if (i < 0) break;
-      chosen |= 1ull << i;
+      kept |= 1ull << i;
     }
-    for (int e = lane; e < E; e += 32)
-      if (!(chosen >> (e / per) & 1ull)) key[e] = -INFINITY;
-    __syncwarp();
   }
+  // the keys: score + bias, or the logits
+  for (int e = lane; e < E; e += 32) {
+    const float x = mx_to_f32(lg[e]);
+    if (!bias && val[e] != -INFINITY) val[e] = x != x ? -DBL_MAX : (double)x;
+    if (!(kept >> (e / per) & 1ull)) val[e] = -INFINITY;
+  }
+  __syncwarp();
   int mine = -1;
-  for (int k = 0; k < K; ++k) {
+  for (int k = 0; k < a.K; ++k) {
     double v = 0;
     int i = -1;
     for (int e = lane; e < E; e += 32)
-      if (key[e] != -INFINITY && (i < 0 || key[e] > v)) {
-        v = key[e];
+      if (val[e] != -INFINITY && (i < 0 || val[e] > v)) {
+        v = val[e];
         i = e;
       }
     warp_best(v, i);
     if (i < 0) break;
     if (lane == k) mine = i;
-    if ((i & 31) == lane) key[i] = -INFINITY;
+    if ((i & 31) == lane) val[i] = -INFINITY;
     __syncwarp();
   }
   return mine;
@@ -117,303 +149,382 @@ __device__ __forceinline__ void load_chunk(const T* p, int e0, int E, bool vec, 
   }
 }
 
-// Order-preserving map of a number to an unsigned key >= 2; NaN gives 1, masked entries use 0.
+// Order-preserving map of a number to an unsigned key; a masked entry is 0, below all of them.
 __device__ __forceinline__ unsigned order_key(float v) {
-  v += 0.f;                                       // -0 -> +0
   const unsigned b = __float_as_uint(v);
-  return v != v ? 1u : b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
+  return b ^ ((unsigned)((int)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(unsigned k) {
   return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
 }
 
-// A row's selection with 64-bit keys (shared memory: key[E], value[E], gscore[64]).
-template <typename T>
-__device__ __noinline__ int select_row64(const RouteArgs& a, const T* lg, const float* bias, double* key, int lane) {
-  const int E = a.E;
-  double* value = key + E;
-  double* gscore = value + E;
-  if (a.score_func == 0) {
-    float m = -INFINITY;
-    bool nan = false;
-    for (int e = lane; e < E; e += 32) {
-      const float x = mx_to_f32(lg[e]);
-      nan |= x != x;
-      m = fmaxf(m, x);
-    }
+// Descending sort of a thread's keys: Batcher's odd-even merge network (Batcher 1968).
+template <int N>
+__device__ __forceinline__ void sort_keys(unsigned (&k)[N]) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-    if (__any_sync(FULL, nan)) m = NAN;
-    double sum = 0;
-    for (int e = lane; e < E; e += 32) sum += exp((double)mx_to_f32(lg[e]) - (double)m);
-    sum = warp_sum(sum);
-    for (int e = lane; e < E; e += 32) value[e] = exp((double)mx_to_f32(lg[e]) - (double)m) / sum;
-  } else {
-    for (int e = lane; e < E; e += 32) value[e] = 1.0 / (1.0 + exp(-(double)mx_to_f32(lg[e])));
-  }
-  for (int e = lane; e < E; e += 32) {
-    const float x = mx_to_f32(lg[e]);
-    const float b = bias ? bias[e] : 0.f;
-    const bool masked = x == -INFINITY || b == -INFINITY;
-    double v = value[e] + (double)b;
-    if (v != v) v = -DBL_MAX;
-    const double kx = bias ? v : (x != x ? -DBL_MAX : (double)x);
-    value[e] = masked ? -INFINITY : v;
-    key[e] = masked ? -INFINITY : kx;
-  }
-  __syncwarp();
-  return select64(key, value, gscore, E, a.K, a.groups, a.keep, lane);
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int q = p; q >= 1; q /= 2)
+#pragma unroll
+      for (int j = q % p; j < N - q; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (i + j + q < N && (i + j) / (2 * p) == (i + j + q) / (2 * p)) {
+            const unsigned hi = max(k[i + j], k[i + j + q]), lo = min(k[i + j], k[i + j + q]);
+            k[i + j] = hi;
+            k[i + j + q] = lo;
+          }
 }
 
-// Lane l holds experts [l * NPL, (l + 1) * NPL) in registers.  Keys are fp32; where two candidates
-// whose order matters are closer than the keys' error (and are not the same logit and bias),
-// the row's selection is done again in 64 bits.  Bounds of that error: a softmax score is off by
-// less than 2^-18 of the row's largest score (sum, exponent argument and exponential), a
-// sigmoid by less than 2^-21, the sum with the bias by half a unit of 2^-23; a difference of two is
-// off by twice that, of two group sums by four times.
+// Bytes of shared memory a warp needs: 64-bit keys and group scores of a row done again, which
+// also hold the lanes' sorted keys (32 (NPL + 1) words <= 8 E + 512).
+__host__ __device__ constexpr int fwd_scratch_bytes(int E) { return 8 * E + 512; }
+
+// A warp takes `rpw` consecutive rows one after another; what follows the selection (scores of the
+// chosen, normalisation, stores) is done for all of them at once, seg = 32 / rpw >= K lanes a row.
+//
+// Lane l holds experts [l * NPL, (l + 1) * NPL) of the row in registers.  A key is the order-preserving map of
+// the candidate's fp32 value with its low bits replaced by the complement of the expert's id:
+// keys are unique, equal values rank by id, and one warp-wide integer maximum gives the best
+// value and its id.  Each lane sorts its keys once and offers its largest.
+//
+// The bits given up and fp32 scores can put close candidates in the wrong order.  So the chosen
+// ones are compared once more by their full fp32 values, and the last of them with the largest
+// value the first one left out can have; where a gap is not above the values' error (and the
+// two are not the same logit and bias) the row is selected again in 64 bits.  Bounds of the
+// error: a softmax score is off by less than 2^-18 of the row's largest score (sum, exponent
+// argument and exponential), a sigmoid by less than 2^-21, the sum with the bias by half a unit
+// of 2^-23; a difference of two by twice that, of two group sums by four times.  Logits
+// themselves (no bias) are exact: 16-bit ones fit above the id bits, so their keys are too.
 template <int DT, int NPL>
-__global__ void __launch_bounds__(RE_WARPS * 32)
-    route_experts_kernel(const RouteArgs a, bool vec, unsigned per_magic, float* __restrict__ weights,
-                         int64_t* __restrict__ idx, float* __restrict__ saved) {
+__global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 : 4)
+    route_experts_kernel(const __grid_constant__ RouteArgs a, bool vec, unsigned per_magic, int rpw,
+                         float* __restrict__ weights, int64_t* __restrict__ idx, float* __restrict__ saved) {
   pdl_wait();
   pdl_trigger();
   using T = typename MxType<DT>::T;
+  constexpr unsigned ID = 32 * NPL - 1;                           // id bits of a key
+  constexpr float LOG2E = 1.44269504f;
   extern __shared__ double smd[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned row = blockIdx.x * RE_WARPS + warp;
-  if (row >= (unsigned)(a.H * a.S)) return;
-  const unsigned h = row / (unsigned)a.S, s = row - h * (unsigned)a.S;
-  const int E = a.E, K = a.K, e0 = lane * NPL;
-  const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
-  const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
-  double* scratch = smd + (size_t)warp * (2 * E + 64);
-  int mine = -1;
-  float m = 0.f, sum = 1.f;
-  if (!a.token_mask || a.token_mask[h * a.mask_stride_h + s]) {
+  const unsigned rows = (unsigned)(a.H * a.S), row0 = (blockIdx.x * RE_WARPS + warp) * (unsigned)rpw;
+  if (row0 >= rows) return;
+  const int n_rows = (int)min((unsigned)rpw, rows - row0), seg = 32 / rpw;
+  const int E = a.E, K = a.K, e0 = lane * NPL, G = a.groups;
+  const bool grouped = a.keep < G, exact = DT != DT_F32 && !a.bias;
+  double* scratch = smd + (size_t)warp * (fwd_scratch_bytes(E) / 8);
+  // of this lane's choice (row row0 + lane / seg, rank lane % seg)
+  unsigned mine_key = 0, extra = 0;
+  float m_l = 0.f, sum_l = 1.f, tol_l = 0x1p-20f;
+  bool close = false;
+  unsigned h = row0 / (unsigned)a.S, s = row0 - h * (unsigned)a.S;
+  for (int r = 0; r < n_rows; ++r, ++s) {
+    if (s == (unsigned)a.S) {
+      s = 0;
+      ++h;
+    }
+    if (a.token_mask && !a.token_mask[h * a.mask_stride_h + s]) continue;
+    const bool mine_row = lane / seg == r;
+    const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
+    const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
     float x[NPL];
     load_chunk<T, NPL>(lg, e0, E, vec, -INFINITY, x);
-    float smax = 1.f;
+    // infinities and NaN make a product with 0 that is not 0; lanes that reach over E count too
+    float probe = 0.f;
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) probe = fmaf(x[j], 0.f, probe);
+    const bool special = e0 < E && !(probe == 0.f);
+    float m = 0.f, tol0 = 0x1p-20f;
     if (a.score_func == 0) {
       m = x[0];
-      bool nan = x[0] != x[0];
 #pragma unroll
-      for (int j = 1; j < NPL; ++j) {
-        nan |= x[j] != x[j];
-        m = fmaxf(m, x[j]);
+      for (int j = 1; j < NPL; ++j) m = fmaxf(m, x[j]);
+      bool nan = false;
+      if (special) {
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) nan |= x[j] != x[j];
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
       if (__any_sync(FULL, nan)) m = NAN;
+      if (m == -INFINITY) continue;                               // no expert is left
     }
     unsigned key[NPL];
-    if (a.score_func == 0 && m == -INFINITY) {
-#pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = 0;                   // no expert is left
-    } else {
-      const bool need_v = bias || a.groups > 1;
+    if (bias || grouped || a.score_func == 0) {
       float v[NPL];
       if (a.score_func == 0) {
-        sum = 0.f;
+        float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
-          v[j] = __expf(x[j] - m);
+          v[j] = ex2_approx((x[j] - m) * LOG2E);
           sum += v[j];
         }
         sum = warp_sum(sum);
-        smax = __fdiv_rn(1.f, sum);
+        const float smax = __fdividef(1.f, sum);
+        if (mine_row) {
+          m_l = m;
+          sum_l = sum;
+        }
+        tol0 = smax * 0x1p-17f;
+        if (bias || grouped) {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) v[j] *= smax;
-      } else if (need_v) {
+          for (int j = 0; j < NPL; ++j) v[j] *= smax;
+        }
+      } else {
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) v[j] = __fdividef(1.f, 1.f + __expf(-x[j]));
+        for (int j = 0; j < NPL; ++j) v[j] = rcp_approx(1.f + ex2_approx(x[j] * -LOG2E));
       }
-      bool gone[NPL];
+      if (bias || grouped) {
+        if (bias) {
+          float b[NPL];
+          load_chunk<float, NPL>(bias, e0, E, vec, 0.f, b);
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) gone[j] = x[j] == -INFINITY;
-      if (bias) {
-        float b[NPL];
-        load_chunk<float, NPL>(bias, e0, E, vec, -INFINITY, b);
+          for (int j = 0; j < NPL; ++j) v[j] += b[j];
+        }
 #pragma unroll
-        for (int j = 0; j < NPL; ++j) {
-          gone[j] |= b[j] == -INFINITY;
-          v[j] += b[j];
+        for (int j = 0; j < NPL; ++j) key[j] = order_key(v[j]);
+        // experts without a number: masked ones (a bias may be -inf too) and NaN
+        bool odd = special;
+        if (bias) {
+          float pv = 0.f;
+#pragma unroll
+          for (int j = 0; j < NPL; ++j) pv = fmaf(v[j], 0.f, pv);
+          odd |= !(pv == 0.f);
+        }
+        if (odd) {
+#pragma unroll
+          for (int j = 0; j < NPL; ++j) {
+            if (v[j] != v[j]) key[j] = order_key(-FLT_MAX);
+            if (x[j] == -INFINITY || (bias && e0 + j < E && bias[e0 + j] == -INFINITY)) key[j] = 0;
+          }
         }
       }
+    }
+    unsigned long long kept = ~0ull;
+    if (grouped) {
+      // two best of every group: 32 / G lanes (a power of two) walk a group in shared memory
+      const int per = E / G;
+      unsigned* sv = reinterpret_cast<unsigned*>(scratch);
+      __syncwarp();
 #pragma unroll
-      for (int j = 0; j < NPL; ++j) key[j] = gone[j] ? 0u : order_key(bias ? v[j] : x[j]);
-      const float tol0 = a.score_func == 0 ? smax * 0x1p-17f : 0x1p-20f;
-      bool close = false;                                         // warp-uniform
-      if (a.groups > 1 && a.keep < a.groups) {
-        // two best of every group: 32 / G lanes (a power of two) walk a group in shared memory
-        const int G = a.groups, per = E / G;
-        unsigned* sv = reinterpret_cast<unsigned*>(scratch);
+      for (int j = 0; j < NPL; ++j)
+        if (e0 + j < E) sv[e0 + j] = key[j];
+      __syncwarp();
+      const int lanes = G > 16 ? 1 : G > 8 ? 2 : G > 4 ? 4 : G > 2 ? 8 : 16;
+      unsigned gk[2];
+      float mag = 0.f;                                            // bounds the roundings of v: sums may cancel
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int g = lane / lanes + 32 * half;
+        unsigned b1 = 0, b2 = 0;
+        if (g < G)
+          for (int i = lane & (lanes - 1); i < per; i += lanes) {
+            const unsigned k = sv[g * per + i];
+            b2 = max(b2, min(b1, k));
+            b1 = max(b1, k);
+          }
+        for (int o = 1; o < lanes; o <<= 1) {
+          const unsigned o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
+          b2 = max(max(b2, o2), min(b1, o1));
+          b1 = max(b1, o1);
+        }
+        const float v1 = key_value(b1), v2 = b2 ? key_value(b2) : 0.f;
+        if (b1) mag = fmaxf(mag, fabsf(v1) + fabsf(v2));
+        // unique keys again: the group's id in the low six bits
+        gk[half] = b1 == 0 || (lane & (lanes - 1)) ? 0u : (order_key(v1 + v2) & ~63u) | (63u - g);
+        if (G <= 32) {
+          gk[1] = 0;
+          break;
+        }
+      }
+      mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(mag)));
+      kept = 0;
+      unsigned last = 0, best = __reduce_max_sync(FULL, max(gk[0], gk[1]));
+      for (int t = 0; t < a.keep && best; ++t) {
+        kept |= 1ull << (63u - (best & 63u));
+        gk[0] = gk[0] == best ? 0u : gk[0];
+        gk[1] = gk[1] == best ? 0u : gk[1];
+        last = best;
+        best = __reduce_max_sync(FULL, max(gk[0], gk[1]));
+      }
+      if (best) close |= mine_row && !(key_value(last & ~63u) - key_value(best | 63u) > 4.f * tol0 + 0x1p-21f * mag);
+      __syncwarp();
+    }
+    if (!bias) {
+      if (special) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
-          if (e0 + j < E) sv[e0 + j] = gone[j] ? 0u : order_key(v[j]);
-        __syncwarp();
-        const int lanes = G > 16 ? 1 : G > 8 ? 2 : G > 4 ? 4 : G > 2 ? 8 : 16;
-        unsigned gk[2];
-        float mag = 0.f;                                          // bounds the roundings of v: sums may cancel
+          key[j] = x[j] == -INFINITY ? 0u : order_key(x[j] != x[j] ? -FLT_MAX : x[j] + 0.f);
+      } else {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int g = lane / lanes + 32 * half;
-          unsigned b1 = 0, b2 = 0;
-          if (g < G)
-            for (int i = lane & (lanes - 1); i < per; i += lanes) {
-              const unsigned k = sv[g * per + i];
-              b2 = max(b2, min(b1, k));
-              b1 = max(b1, k);
-            }
-          for (int o = 1; o < lanes; o <<= 1) {
-            const unsigned o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
-            b2 = max(max(b2, o2), min(b1, o1));
-            b1 = max(b1, o1);
-          }
-          close |= b1 == 1u || b2 == 1u;                          // a NaN among the two best
-          if (b1 > 1u) mag = fmaxf(mag, fabsf(key_value(b1)) + (b2 > 1u ? fabsf(key_value(b2)) : 0.f));
-          const float total = b2 ? key_value(b1) + key_value(b2) : key_value(b1);
-          gk[half] = b1 == 0 || (lane & (lanes - 1)) ? 0u : order_key(total);
-          if (G <= 32) {
-            gk[1] = 0;
-            break;
-          }
-        }
-        close = __any_sync(FULL, close);
-        mag = __uint_as_float(__reduce_max_sync(FULL, __float_as_uint(mag)));
-        unsigned long long kept = 0;
-        unsigned last = 0;
-        for (int t = 0; t <= a.keep; ++t) {
-          const unsigned best = __reduce_max_sync(FULL, max(gk[0], gk[1]));
-          if (best == 0) break;
-          if (t == a.keep) {
-            const float lv = key_value(last);
-            close |= !(lv - key_value(best) > 4.f * tol0 + 0x1p-21f * mag);
-            break;
-          }
-          const unsigned in0 = __ballot_sync(FULL, gk[0] == best), in1 = __ballot_sync(FULL, gk[1] == best);
-          const int owner = __ffs(in0 ? in0 : in1) - 1;
-          kept |= 1ull << (in0 ? owner / lanes : owner + 32);
-          if (lane == owner) gk[in0 ? 0 : 1] = 0;
-          last = best;
-        }
+        for (int j = 0; j < NPL; ++j) key[j] = order_key(x[j] + 0.f);        // -0 ranks as 0
+      }
+    }
+    if (grouped) {
+      const int g0 = (int)((e0 * per_magic) >> 20), per = E / G;
+      if (per >= NPL) {                                           // a lane's experts lie in two groups at most
+        const bool in0 = kept >> (g0 & 63) & 1ull, in1 = kept >> ((g0 + 1) & 63) & 1ull;
+        const int edge = (g0 + 1) * per - e0;
+#pragma unroll
+        for (int j = 0; j < NPL; ++j) key[j] = (j < edge ? in0 : in1) ? key[j] : 0u;
+      } else {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
           if (!(kept >> ((((e0 + j) * per_magic) >> 20) & 63u) & 1ull)) key[j] = 0;
       }
-      // K rounds: the best lane wins, the lower lane (and expert) among equals; one more round
-      // shows how close the first one left out is
-      unsigned top = 0, next = 0;
-      int tj = 0, mine_next = -1;
-      auto local_best = [&] {
-        top = 0;
+    }
+    const unsigned high = e0 < E ? ~ID : 0u;
 #pragma unroll
-        for (int j = 0; j < NPL; ++j)
-          if (key[j] > top) {
-            top = key[j];
-            tj = j;
-          }
-      };
-      local_best();
-      unsigned mine_key = 0;
-      const int rounds = bias ? K + 1 : K;
-      for (int k = 0; k < rounds; ++k) {
-        const unsigned best = __reduce_max_sync(FULL, top);
-        if (best == 0) break;
-        const int owner = __ffs(__ballot_sync(FULL, top == best)) - 1;
-        const int id = owner * NPL + __shfl_sync(FULL, tj, owner);
-        if (lane == k && k < K) {
-          mine = id;
-          mine_key = best;
-        }
-        if (lane == k - 1) {
-          mine_next = id;
-          next = best;
-        }
-        if (lane == owner) {
+    for (int j = 0; j < NPL; ++j) key[j] = (key[j] & high) | (ID - e0 - j);
+    sort_keys(key);
+    unsigned* list = reinterpret_cast<unsigned*>(scratch) + lane;
 #pragma unroll
-          for (int j = 0; j < NPL; ++j)
-            if (j == tj) key[j] = 0;
-          local_best();
-        }
-      }
-      if (bias) {
-        bool mine_close = false;
-        if (mine >= 0 && mine_next >= 0) {
-          const float v0 = key_value(mine_key), v1 = key_value(next);
-          if (!(v0 - v1 > tol0 + 0x1p-22f * fabsf(v0)) || next == 1u)
-            mine_close = mx_to_f32(lg[mine]) != mx_to_f32(lg[mine_next]) || bias[mine] != bias[mine_next];
-        }
-        close |= __any_sync(FULL, mine_close);
-      }
-      if (close) {
-        __syncwarp();
-        mine = select_row64<T>(a, lg, bias, scratch, lane);
+    for (int j = 0; j < NPL; ++j) list[j * 32] = key[j];
+    list[NPL * 32] = 0;
+    // K rounds, and one more that shows the first one left out; what is left when nothing is, are
+    // bare ids, and 0 behind them, which is not taken off
+    unsigned top = key[0];
+    int slot = r * seg - lane;
+#pragma unroll 4
+    for (int k = 0; k < K; ++k, ++slot) {
+      const unsigned best = __reduce_max_sync(FULL, top);
+      mine_key = slot == 0 ? best : mine_key;
+      list += top == best && best ? 32 : 0;
+      top = *list;
+    }
+    if (!exact) {
+      const unsigned best = __reduce_max_sync(FULL, top);
+      extra = mine_row && best > ID ? best : extra;
+    }
+    if (mine_row) tol_l = tol0;
+  }
+
+  // each lane its own choice
+  const int rank = lane % seg;
+  const unsigned row = row0 + lane / seg;
+  const bool live = lane / seg < n_rows && rank < K;
+  h = row / (unsigned)a.S;
+  s = row - h * (unsigned)a.S;
+  const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
+  const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
+  int mine = mine_key > ID ? (int)(ID - (mine_key & ID)) : -1;
+  float x = 0.f, p = 0.f, b = 0.f;
+  auto score = [&] {
+    p = 0.f;
+    if (mine >= 0) {
+      x = mx_to_f32(lg[mine]);
+      p = a.score_func == 0 ? __fdiv_rn(expf(x - m_l), sum_l) : __fdiv_rn(1.f, 1.f + expf(-x));
+    }
+  };
+  score();
+  if (!exact) {
+    if (bias && mine >= 0) b = bias[mine];
+    const float v = bias ? p + b : x;
+    const float tol = bias ? tol_l + 0x1p-22f * fabsf(v) : 0.f;
+    const float v1 = __shfl_down_sync(FULL, v, 1), x1 = __shfl_down_sync(FULL, x, 1), b1 = __shfl_down_sync(FULL, b, 1);
+    const bool next = __shfl_down_sync(FULL, mine, 1) >= 0;
+    if (mine >= 0) {
+      if (rank + 1 < K) {
+        if (next) close |= !(v - v1 > tol) && !(x == x1 && b == b1);
+      } else if (extra) {
+        close |= !(v - key_value(extra | ID) > tol);
       }
     }
   }
-  float p = 0.f, keep_for_bwd = 0.f;
-  if (mine >= 0) {
-    const float x = mx_to_f32(lg[mine]);
-    p = a.score_func == 0 ? __fdiv_rn(expf(x - m), sum) : __fdiv_rn(1.f, 1.f + expf(-x));
-    keep_for_bwd = a.score_func == 0 ? p : x;
+  for (unsigned again = __ballot_sync(FULL, close && live); again;) {
+    const int r = (__ffs(again) - 1) / seg;
+    again &= seg == 32 ? 0u : ~(((1u << seg) - 1u) << (r * seg));
+    __syncwarp();
+    const unsigned rr = row0 + r, hr = rr / (unsigned)a.S;
+    const int id = select_row64<T>(a, static_cast<const T*>(a.logits) + hr * a.stride_h + (rr - hr * a.S) * a.stride_s,
+                                   a.bias ? a.bias + (int64_t)hr * E : nullptr, scratch, lane);
+    const int got = __shfl_sync(FULL, id, rank);
+    if (lane / seg == r) {
+      mine = got;
+      score();
+    }
   }
   float w = p;
   if (a.route_norm) {
-    const float n = warp_sum(p);
+    float n = p;
+    for (int o = seg / 2; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
     w = __fdiv_rn(p, n != n ? n : fmaxf(n, a.norm_eps));
   }
-  if (lane < K) {
-    const int64_t o = (int64_t)row * K + lane;
+  if (live) {
+    const int64_t o = (int64_t)row * K + rank;
     weights[o] = w * a.route_scale;
     idx[o] = mine;
-    if (saved) saved[o] = keep_for_bwd;
+    if (saved) saved[o] = a.score_func == 0 ? p : x;
   }
 }
 
-// One warp per row; the row's gradient is put together in shared memory (most of it zero) and
-// stored in order, NPL experts a lane.
+// `rpw` rows a warp, seg = 32 / rpw >= K lanes a row for the chosen experts.  A row's gradient is zero
+// but for the chosen ones (sigmoid, or softmax with the norm): rows are cleared with wide stores
+// and the chosen entries stored over them.  The other rows (softmax where the norm does not
+// cancel the common term) are written by the whole warp, dl = -score (sum ds p), and the chosen
+// entries, p (ds - sum ds p), over them.
 template <int DT, int NPL>
 __global__ void __launch_bounds__(RE_WARPS * 32)
-    route_experts_bwd_kernel(const RouteArgs a, bool vec, bool vec_out, const float* __restrict__ grad_w, int64_t gs_h,
-                             int64_t gs_s, const int64_t* __restrict__ idx, const float* __restrict__ saved,
+    route_experts_bwd_kernel(const __grid_constant__ RouteArgs a, bool vec, bool vec_out, int rpw,
+                             const float* __restrict__ grad_w, int64_t gs_h, int64_t gs_s,
+                             const int64_t* __restrict__ idx, const float* __restrict__ saved,
                              typename MxType<DT>::T* __restrict__ dl) {
   pdl_wait();
   pdl_trigger();
   using T = typename MxType<DT>::T;
-  extern __shared__ float smf[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned row = blockIdx.x * RE_WARPS + warp;
-  if (row >= (unsigned)(a.H * a.S)) return;
+  const unsigned rows = (unsigned)(a.H * a.S), row0 = (blockIdx.x * RE_WARPS + warp) * (unsigned)rpw;
+  if (row0 >= rows) return;
+  const int n_rows = (int)min((unsigned)rpw, rows - row0), seg = 32 / rpw;
+  const int E = a.E, K = a.K, rank = lane % seg;
+  const unsigned row = row0 + lane / seg;
+  const bool live = lane / seg < n_rows && rank < K;
   const unsigned h = row / (unsigned)a.S, s = row - h * (unsigned)a.S;
-  const int E = a.E, K = a.K, e0 = lane * NPL;
-  float* d = smf + (size_t)warp * (32 * NPL);
-  const int64_t id = lane < K ? idx[(int64_t)row * K + lane] : -1;
+  const int64_t id = live ? idx[(int64_t)row * K + rank] : -1;
   const bool has = id >= 0 && id < E;
   float p = 0.f, q = 0.f, g = 0.f;
   if (has) {
-    p = saved[(int64_t)row * K + lane];
-    g = grad_w[h * gs_h + s * gs_s + lane] * a.route_scale;
+    p = saved[(int64_t)row * K + rank];
+    g = grad_w[h * gs_h + s * gs_s + rank] * a.route_scale;
     if (a.score_func == 1) {
       q = __fdiv_rn(1.f, 1.f + expf(p));
       p = __fdiv_rn(1.f, 1.f + expf(-p));
     }
   }
+  auto seg_sum = [&](float v) {
+    for (int o = seg / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
+    return v;
+  };
   float ds = g;
-  bool zero_dot = false;
+  bool cancels = false;                                           // the softmax's common term is 0
   if (a.route_norm) {
-    const float n = warp_sum(p);
-    const float gp = warp_sum(g * p);
+    const float n = seg_sum(p), gp = seg_sum(g * p);
     const float den = n != n ? n : fmaxf(n, a.norm_eps);
-    zero_dot = n > a.norm_eps;
+    cancels = n > a.norm_eps;
     ds = __fdiv_rn(g, den);
-    if (zero_dot) ds = __fdiv_rn(g - __fdiv_rn(gp, den), den);
+    if (cancels) ds = __fdiv_rn(g - __fdiv_rn(gp, den), den);
   }
-  float o[NPL];
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) o[j] = 0.f;
-  if (a.score_func == 0 && !zero_dot && __any_sync(FULL, has)) {
-    const float dot = warp_sum(has ? ds * p : 0.f);
-    const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
+  const bool dense_row = a.score_func == 0 && !cancels;
+  const float dot = seg_sum(has && dense_row ? ds * p : 0.f);
+  const unsigned dense = a.score_func == 0 ? __ballot_sync(FULL, dense_row && has) : 0u;
+  const unsigned sparse = __ballot_sync(FULL, live && !dense_row) | __ballot_sync(FULL, live && !has);
+  T* out = dl + (int64_t)row0 * E;
+  if (sparse) {
+    const int64_t n = (int64_t)n_rows * E;
+    constexpr int W = 16 / (int)sizeof(T);
+    const int64_t wide = vec_out ? n / W : 0;
+    for (int64_t i = lane; i < wide; i += 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0, 0, 0, 0);
+    for (int64_t i = wide * W + lane; i < n; i += 32) mx_store(out + i, 0.f);
+  }
+  __syncwarp();
+  for (unsigned todo = dense; todo;) {
+    const int r = (__ffs(todo) - 1) / seg;
+    todo &= seg == 32 ? 0u : ~(((1u << seg) - 1u) << (r * seg));
+    const unsigned rr = row0 + r, hr = rr / (unsigned)a.S;
+    const T* lg = static_cast<const T*>(a.logits) + hr * a.stride_h + (rr - hr * a.S) * a.stride_s;
+    const float row_dot = __shfl_sync(FULL, dot, r * seg);
+    const int e0 = lane * NPL;
+    float o[NPL];
     load_chunk<T, NPL>(lg, e0, E, vec, -INFINITY, o);
     float m = o[0], sum = 0.f;
 #pragma unroll
@@ -425,31 +536,24 @@ __global__ void __launch_bounds__(RE_WARPS * 32)
       o[j] = o[j] == -INFINITY ? 0.f : expf(o[j] - m);
       sum += o[j];
     }
-    const float f = -__fdiv_rn(dot, warp_sum(sum));
-#pragma unroll
-    for (int j = 0; j < NPL; ++j) o[j] = o[j] == 0.f ? 0.f : o[j] * f;
-  }
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) d[j * 32 + lane] = o[j];          // expert e at (e % NPL) * 32 + e / NPL
-  __syncwarp();
-  if (has) d[(int)(id % NPL) * 32 + (int)(id / NPL)] += a.score_func == 0 ? ds * p : ds * p * q;
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < NPL; ++j) o[j] = d[j * 32 + lane];
-  T* out = dl + (int64_t)row * E + e0;
-  if (vec_out && e0 + NPL <= E) {
+    const float f = -__fdiv_rn(row_dot, warp_sum(sum));
+    T* dst = out + (int64_t)r * E + e0;
     constexpr int BYTES = NPL * (int)sizeof(T);
     struct alignas(BYTES < 16 ? BYTES : 16) Chunk {
       T v[NPL];
     } c;
 #pragma unroll
-    for (int j = 0; j < NPL; ++j) mx_store(&c.v[j], o[j]);
-    *reinterpret_cast<Chunk*>(out) = c;
-  } else {
+    for (int j = 0; j < NPL; ++j) mx_store(&c.v[j], o[j] == 0.f ? 0.f : o[j] * f);
+    if (vec && e0 + NPL <= E) {
+      *reinterpret_cast<Chunk*>(dst) = c;
+    } else {
 #pragma unroll
-    for (int j = 0; j < NPL; ++j)
-      if (e0 + j < E) mx_store(out + j, o[j]);
+      for (int j = 0; j < NPL; ++j)
+        if (e0 + j < E) dst[j] = c.v[j];
+    }
   }
+  __syncwarp();
+  if (has) mx_store(dl + (int64_t)row * E + id, a.score_func == 1 ? ds * p * q : p * (ds - dot));
 }
 
 // Experts a lane: the smallest power of two that covers E with 32 lanes.
@@ -466,10 +570,19 @@ bool chunks_aligned(const void* p, int64_t stride_h, int64_t stride_s, int E, in
          stride_s * esz % unit == 0;
 }
 
+// Rows a warp takes: as many as have K lanes each, while 16 warps a SM are left.
+int rows_per_warp(int64_t rows, int K) {
+  int rpw = 1;
+  while (2 * rpw * K <= 32 && rpw < 8 && rows >= (int64_t)num_sms() * 16 * rpw * 2) rpw *= 2;
+  return rpw;
+}
+
 template <int DT, int NPL>
 cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)a.H * a.S + RE_WARPS - 1) / RE_WARPS);
-  const size_t smem = (size_t)RE_WARPS * (2 * a.E + 64) * sizeof(double);
+  const int64_t rows = (int64_t)a.H * a.S;
+  const int rpw = rows_per_warp(rows, a.K);
+  const unsigned grid = (unsigned)((rows + RE_WARPS * rpw - 1) / (RE_WARPS * rpw));
+  const size_t smem = (size_t)RE_WARPS * fwd_scratch_bytes(a.E);
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(route_experts_kernel<DT, NPL>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -479,19 +592,23 @@ cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* sav
                    (!a.bias || chunks_aligned(a.bias, a.E, 0, a.E, 4, NPL));
   // e / per = e * ceil(2^20 / per) >> 20 for e < 1024
   const unsigned per = (unsigned)(a.E / a.groups), magic = ((1u << 20) + per - 1) / per;
-  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL>), grid, RE_WARPS * 32, smem, st, a, vec, magic, weights, idx, saved);
+  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL>), grid, RE_WARPS * 32, smem, st, a, vec, magic, rpw, weights, idx, saved);
   return cudaGetLastError();
 }
 
 template <int DT, int NPL>
 cudaError_t run_bwd(const RouteArgs& a, const float* grad_w, int64_t gs_h, int64_t gs_s, const int64_t* idx,
                     const float* saved, void* dl, cudaStream_t st) {
-  const unsigned grid = (unsigned)(((int64_t)a.H * a.S + RE_WARPS - 1) / RE_WARPS);
+  const int64_t rows = (int64_t)a.H * a.S;
+  const int rpw = rows_per_warp(rows, a.K);
+  const unsigned grid = (unsigned)((rows + RE_WARPS * rpw - 1) / (RE_WARPS * rpw));
   constexpr int esz = DT == DT_F32 ? 4 : 2;
-  const bool vec = a.logits && chunks_aligned(a.logits, a.stride_h, a.stride_s, a.E, esz, NPL);
-  const bool vec_out = chunks_aligned(dl, 0, a.E, a.E, esz, NPL);
-  MHMOE_LAUNCH_PDL((route_experts_bwd_kernel<DT, NPL>), grid, RE_WARPS * 32, (size_t)RE_WARPS * 32 * NPL * 4, st, a, vec,
-                   vec_out, grad_w, gs_h, gs_s, idx, saved, static_cast<typename MxType<DT>::T*>(dl));
+  // dense rows: logits and gradient in the same chunks; cleared rows: 16-B stores from the warp's first
+  const bool vec = a.logits && chunks_aligned(a.logits, a.stride_h, a.stride_s, a.E, esz, NPL) &&
+                   chunks_aligned(dl, 0, a.E, a.E, esz, NPL);
+  const bool vec_out = reinterpret_cast<uintptr_t>(dl) % 16 == 0 && (int64_t)rpw * a.E * esz % 16 == 0;
+  MHMOE_LAUNCH_PDL((route_experts_bwd_kernel<DT, NPL>), grid, RE_WARPS * 32, 0, st, a, vec, vec_out, rpw, grad_w, gs_h,
+                   gs_s, idx, saved, static_cast<typename MxType<DT>::T*>(dl));
   return cudaGetLastError();
 }
 
