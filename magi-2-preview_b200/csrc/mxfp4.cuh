@@ -186,11 +186,23 @@ __device__ __forceinline__ void mx_decode8(uint32_t w, float (&v)[8]) {
   }
 }
 
-// SwiGLU7: min(g, 7) * sigmoid(1.702 min(g, 7)) * (clamp(u, -7, 7) + 1); NaN goes through.
+// SwiGLU7: min(g, 7) * sigmoid(1.702 min(g, 7)) * (clamp(u, -7, 7) + 1); NaN goes through.  2^x and
+// 1/x are the special-function unit's, each off by two units of 2^-23 at most; where they flush
+// to 0 or overflow, |g sigmoid| is below 2^-100.
+__device__ __forceinline__ float mx_min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float mx_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float mx_swiglu7(float g, float u) {
-  g = g > 7.f ? 7.f : g;
-  u = u > 7.f ? 7.f : (u < -7.f ? -7.f : u);
-  return __fdividef(g, 1.f + __expf(-1.702f * g)) * (u + 1.f);
+  g = mx_min_nan(g, 7.f);
+  u = mx_max_nan(mx_min_nan(u, 7.f), -7.f);
+  return g * rcp_approx(1.f + ex2_approx(g * (-1.702f * 1.44269504f))) * (u + 1.f);
 }
 
 // mxfp4.cu

@@ -8,49 +8,59 @@
 // of token tiles).  The second, mx_gemm_kernel, multiplies on the tensor cores
 // (tcgen05.mma kind::mxf4, fp32 accumulators in TMEM).
 //
-// A work item is (token tile, weight tile).  Two orientations share the main loop:
-//   wide   A = 128 token rows, B = 256 weight rows: the most math per operand byte
-//   flat   A = 128 weight rows, B = 16..128 token rows: a few tokens still fill the
-//          instruction's 128 lanes with weights, which is what a decode step streams
+// A work item is (token tile, weight tile), in one of two kernels:
+//   wide   256 tokens x 256 weight rows on a pair of CTAs (cta_group::2): 128 tokens a CTA, each
+//          loads half of the weight rows.  One CTA alone would read 51 KB a stage (256 columns)
+//          through a 64 B/clk port, 800 clocks for 549 of MMA; the pair reads 35 KB each.
+//   flat   128 weight rows x 16..128 tokens: with a few tokens the instruction's 128 lanes are
+//          filled by the weights, which is what a decode step streams.  A cluster may share an
+//          item along the columns.
 // Warp roles: 0 TMA producer, 1 TMEM owner and MMA issuer, then the epilogue warps, last the
-// copier of scale atoms into TMEM (their own warp, so that copies run beside the MMAs).  One
-// stage is 256 columns (128 B a row) of both operands with their scale atoms.
+// copier of scale atoms into TMEM (their own warp, so that copies run beside the MMAs).
 #include "mxfp4.cuh"
 
 namespace mhmoe {
 
 namespace {
 
-constexpr int MG_BM = 128;                  // rows of operand A
-constexpr int MG_BK = 256;                  // columns of a stage
+constexpr int MG_BM = 128;                  // rows of operand A a CTA
+constexpr int MG_BK = 256;                  // columns of a stage: 128 B a row
 constexpr int MG_A_BYTES = MG_BM * MG_BK / 2;
-constexpr int MG_SFA_BYTES = 2 * 512;       // two atoms: 128 rows x 256 columns
-constexpr int MG_STG_BYTES = 2048;          // store staging per epilogue warp (wide): 32 rows x 64 B
+constexpr int MG_SF_BYTES = 2 * 512;        // scales of 128 rows x 256 columns: two atoms
+constexpr int MG_STG_BYTES = 2048;          // store staging per epilogue warp: 32 rows x 64 B
 constexpr int MG_MISC_BYTES = 512;          // barriers, TMEM slot
 constexpr int MG_TMEM_COLS = 512;
 
-template <bool FLAT, int BN>
-struct MgShape {
-  static constexpr int NBLK = (BN + 127) / 128;                 // 128-row atom blocks of operand B
-  static constexpr int B_BYTES = BN * MG_BK / 2;
-  static constexpr int SFB_BYTES = NBLK * MG_SFA_BYTES;
-  static constexpr int STAGE = MG_A_BYTES + B_BYTES + MG_SFA_BYTES + SFB_BYTES;
-  static constexpr int EPW = FLAT ? 4 : 8;                      // epilogue warps
-  static constexpr int STG = FLAT ? 0 : EPW * MG_STG_BYTES;
-  static constexpr int STAGES = FLAT ? (BN <= 16 ? 10 : BN <= 32 ? 9 : BN <= 64 ? 8 : 6) : 4;
-  static constexpr int SMEM = STAGES * STAGE + STG + MG_MISC_BYTES + 1024;
+struct WideShape {
+  static constexpr int SLOT = 256, WROWS = 256;                 // tokens and weight rows of a tile
+  static constexpr int B_BYTES = MG_BM * MG_BK / 2;             // half of the weight rows
+  static constexpr int STAGE = MG_A_BYTES + B_BYTES + 3 * MG_SF_BYTES;
+  static constexpr int STAGES = 5;
+  static constexpr int EPW = 16;                                // epilogue warps: 64 columns each
   static constexpr int THREADS = 32 * (3 + EPW);
-  static constexpr int NACC = FLAT ? 2 : 1;                     // accumulators in TMEM
-  static constexpr int SF_COLS = 8 + 8 * NBLK;                  // TMEM columns of a stage's scales
-  static constexpr int SF_COL0 = NACC * BN;
-  static constexpr int SLOT = FLAT ? BN : MG_BM;                // token rows of a tile
-  static constexpr int WROWS = FLAT ? MG_BM : BN;               // weight rows of a tile
+  static constexpr int SMEM = STAGES * STAGE + EPW * MG_STG_BYTES + MG_MISC_BYTES + 1024;
+  static constexpr int SF_COLS = 24, SF_COL0 = 256;             // TMEM: accumulator, then the stages' scales
+  static_assert(SMEM <= 227 * 1024, "shared memory");
+  static_assert(SF_COL0 + STAGES * SF_COLS <= MG_TMEM_COLS, "TMEM");
+};
+
+template <int BN>
+struct FlatShape {
+  static constexpr int SLOT = BN, WROWS = MG_BM;
+  static constexpr int B_BYTES = BN * MG_BK / 2;
+  static constexpr int STAGE = MG_A_BYTES + B_BYTES + 2 * MG_SF_BYTES;
+  static constexpr int EPW = BN >= 64 ? 8 : 4;
+  static constexpr int STAGES = BN <= 16 ? 9 : BN <= 32 ? 8 : BN <= 64 ? 7 : 5;
+  static constexpr int THREADS = 32 * (3 + EPW);
+  static constexpr int SMEM = STAGES * STAGE + EPW * MG_STG_BYTES + MG_MISC_BYTES + 1024;
+  static constexpr int NACC = 2;                                // accumulators in TMEM
+  static constexpr int SF_COLS = 16, SF_COL0 = NACC * BN;
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(SF_COL0 + STAGES * SF_COLS <= MG_TMEM_COLS, "TMEM");
 };
 
 struct MgParams {
-  const uint8_t* sf_tok;      // scale atoms of the token tiles, one 128-row block per slot
+  const uint8_t* sf_tok;      // scale atoms of the token tiles, ceil(SLOT / 128) blocks of 128 rows per slot
   const uint8_t* sf_w;
   const int4* tiles;          // grouped: {expert, first row, rows, slot}; null: dense
   const int* n_tiles;         // grouped: their number (device)
@@ -107,38 +117,62 @@ __device__ __forceinline__ void mg_store(void* y, int dtype, int64_t at, float v
   else static_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-// Epilogue of 32 token rows (one a thread) x 128 accumulator columns: 64 B of outputs per row
-// go through the warp's staging (16-B chunks xor-swizzled over row pairs) and leave as whole
-// sectors, 8 rows a store.
+// 32 rows x 64 B of the warp's staging (16-B chunks xor-swizzled over row pairs) to the rows
+// row0 + 0.. of y, `rows` of them, from output column c0; `width` outputs a row are valid.
+template <int ESZ>
+__device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* stg, int64_t row0, int rows, int c0,
+                                              int width, int lane) {
+  uint8_t* y = static_cast<uint8_t*>(p.y);
+  if (p.y_vec) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = i * 8 + (lane >> 2), k = lane & 3;
+      if (row < rows && k * (16 / ESZ) < width)
+        *reinterpret_cast<uint4*>(y + ((row0 + row) * p.y_stride + c0 + k * (16 / ESZ)) * ESZ) =
+            *reinterpret_cast<const uint4*>(stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4));
+    }
+  } else {
+    constexpr int PER = 64 / ESZ;                   // one output a lane, two rows at once in fp32
+    const int col = lane % PER;
+    for (int row = lane / PER; row < rows; row += 32 / PER) {
+      if (col >= width) break;
+      const uint8_t* src = stg + row * 64 + (((col * ESZ >> 4) ^ ((row >> 1) & 3)) << 4) + (col * ESZ & 15);
+      uint8_t* dst = y + ((row0 + row) * p.y_stride + c0 + col) * ESZ;
+      if constexpr (ESZ == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
+      else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
+    }
+  }
+}
+
+// Wide epilogue: 32 token rows (one a thread) x 64 accumulator columns from weight row col0.
 template <bool OUT32, bool SWIGLU>
-__device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, const uint32_t (&r)[128], int col0,
-                                                 int q, int lane, uint8_t* stg) {
+__device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, uint32_t (&r)[64], int col0,
+                                                 int m0, int lane, uint8_t* stg) {
   constexpr int PER = OUT32 ? 16 : 32;              // outputs of a 64-B chunk
   constexpr int ACC = SWIGLU ? 2 * PER : PER;       // accumulator columns behind them
   const int n_out = SWIGLU ? p.N / 2 : p.N;
-  const int m = q * 32 + lane;
-  const float rw = p.row_weights && m < t.rows ? __ldg(p.row_weights + t.row0 + m) : 1.f;
-  const float* bias = p.bias ? p.bias + (int64_t)t.e * p.N : nullptr;
-  const bool half = p.y_dtype == DT_F16;
+  if (p.bias) {
+    const float* bias = p.bias + (int64_t)t.e * p.N + col0;
 #pragma unroll
-  for (int c = 0; c < 128 / ACC; ++c) {
-    const int a0 = col0 + c * ACC;                  // first weight row of the chunk
-    const int o0 = SWIGLU ? a0 / 2 : a0;
+    for (int i = 0; i < 64; ++i)
+      if (col0 + i < p.N) r[i] = __float_as_uint(__uint_as_float(r[i]) + __ldg(bias + i));
+  }
+  const bool half = p.y_dtype == DT_F16;
+  float rw = 1.f;
+  if (p.row_weights && m0 + lane < t.rows) rw = __ldg(p.row_weights + t.row0 + m0 + lane);
+#pragma unroll
+  for (int c = 0; c < 64 / ACC; ++c) {
     float v[PER];
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if constexpr (SWIGLU) {
-        float g = __uint_as_float(r[c * ACC + 2 * i]), u = __uint_as_float(r[c * ACC + 2 * i + 1]);
-        if (bias && a0 + 2 * i < p.N) {
-          g += __ldg(bias + a0 + 2 * i);
-          u += __ldg(bias + a0 + 2 * i + 1);
-        }
-        v[i] = mx_swiglu7(g, u) * rw;
-      } else {
-        float z = __uint_as_float(r[c * ACC + i]);
-        if (bias && a0 + i < p.N) z += __ldg(bias + a0 + i);
-        v[i] = z * rw;
-      }
+      if constexpr (SWIGLU)
+        v[i] = mx_swiglu7(__uint_as_float(r[c * ACC + 2 * i]), __uint_as_float(r[c * ACC + 2 * i + 1]));
+      else
+        v[i] = __uint_as_float(r[c * ACC + i]);
+    }
+    if (p.row_weights) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) v[i] *= rw;
     }
     __syncwarp();                                   // the chunk before has left the staging
 #pragma unroll
@@ -152,71 +186,285 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
       *reinterpret_cast<uint4*>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
-    if (p.y_vec) {
-      constexpr int P16 = PER / 4;                  // outputs of 16 B
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2), k = lane & 3;
-        if (q * 32 + row < t.rows && o0 + k * P16 < n_out) {
-          const uint4 w = *reinterpret_cast<const uint4*>(stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4));
-          const int64_t at = (t.row0 + q * 32 + row) * p.y_stride + o0 + k * P16;
-          *reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.y) + at * (OUT32 ? 4 : 2)) = w;
-        }
-      }
-    } else {
-      // one output a lane (two rows at once in fp32)
-      const int k = OUT32 ? (lane & 15) >> 2 : lane >> 3, b = OUT32 ? (lane & 3) * 4 : (lane & 7) * 2;
-      const int col = o0 + (OUT32 ? (lane & 15) : lane);
-      for (int i = 0; i < (OUT32 ? 16 : 32); ++i) {
-        const int row = OUT32 ? 2 * i + (lane >> 4) : i;
-        if (q * 32 + row >= t.rows || col >= n_out) continue;
-        const uint8_t* src = stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4) + b;
-        const int64_t at = (t.row0 + q * 32 + row) * p.y_stride + col;
-        if constexpr (OUT32) static_cast<uint32_t*>(p.y)[at] = *reinterpret_cast<const uint32_t*>(src);
-        else static_cast<uint16_t*>(p.y)[at] = *reinterpret_cast<const uint16_t*>(src);
-      }
-    }
+    const int o0 = SWIGLU ? (col0 + c * ACC) / 2 : col0 + c * ACC;
+    mg_store_rows<OUT32 ? 4 : 2>(p, stg, t.row0 + m0, min(32, t.rows - m0), o0, n_out - o0, lane);
   }
 }
 
-// Epilogue of one weight row a thread x up to 32 token columns.
-template <int NC>
-__device__ __forceinline__ void mg_flat_columns(const MgParams& p, const MgTile& t, const uint32_t (&r)[NC], int j0,
-                                                int n, float b) {
+// Flat epilogue: one weight row n a thread (32 of the warp's from n0) x NC token columns from j0.
+// The transposed outputs go through the staging in passes of 64 B a token row.
+template <int NC, bool OUT32>
+__device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile& t, const uint32_t (&r)[NC], int j0,
+                                                 int n0, float b, int lane, uint8_t* stg) {
+  using U = typename std::conditional<OUT32, float, uint16_t>::type;
+  constexpr int ESZ = OUT32 ? 4 : 2, PER = 64 / ESZ;
+  const bool half = p.y_dtype == DT_F16;
+  const int rows = min(NC, t.rows - j0);
+  // a row's weight, from the lane that holds it
+  float rw = 1.f;
+  if (p.row_weights && lane < rows) rw = __ldg(p.row_weights + t.row0 + j0 + lane);
+  float v[NC];
 #pragma unroll
   for (int j = 0; j < NC; ++j) {
-    if (j0 + j >= t.rows) break;
-    const int64_t row = t.row0 + j0 + j;
-    const float rw = p.row_weights ? __ldg(p.row_weights + row) : 1.f;
-    const float z = __uint_as_float(r[j]) + b;
-    if (p.act) {
-      const float u = __shfl_xor_sync(0xffffffffu, z, 1);
-      if (!(n & 1) && n < p.N) mg_store(p.y, p.y_dtype, row * p.y_stride + n / 2, mx_swiglu7(z, u) * rw);
-    } else if (n < p.N) {
-      mg_store(p.y, p.y_dtype, row * p.y_stride + n, z * rw);
+    v[j] = __uint_as_float(r[j]) + b;
+    if (p.act) v[j] = mx_swiglu7(v[j], __shfl_down_sync(0xffffffffu, v[j], 1));     // even lanes: (gate, up)
+    if (p.row_weights) v[j] *= __shfl_sync(0xffffffffu, rw, j);
+  }
+  const int n_out = p.act ? p.N / 2 : p.N, o0 = p.act ? n0 / 2 : n0;
+  const int width = p.act ? 16 : 32;                // outputs of the warp a token row
+#pragma unroll
+  for (int c = 0; c < 32 / PER; ++c) {              // fp32 without activation: two passes of 16 outputs
+    if (c * PER >= width) break;
+    const int at = (p.act ? lane >> 1 : lane) - c * PER;
+    __syncwarp();
+    if (at >= 0 && at < PER && !(p.act && (lane & 1))) {
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        U* dst = reinterpret_cast<U*>(stg + j * 64 + (((at * ESZ >> 4) ^ ((j >> 1) & 3)) << 4) + (at * ESZ & 15));
+        if constexpr (OUT32) *dst = v[j];
+        else *dst = (uint16_t)mg_pack16(v[j], 0.f, half);
+      }
     }
+    __syncwarp();
+    mg_store_rows<ESZ>(p, stg, t.row0 + j0, rows, o0 + c * PER, min(width - c * PER, n_out - o0 - c * PER), lane);
   }
 }
 
-// tmT: token rows [R, cols_p/2], box 128 B x SLOT; tmW: weight rows [n * N, cols_p/2], box 128 B x WROWS.
-// SPLIT (flat only): a cluster of CTAs shares one work item along K; their partial
-// accumulators meet in distributed shared memory and are summed in the order of the ranks.
-template <bool FLAT, int BN, bool SPLIT, bool OUT32, bool SWIGLU>
-__global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
-    mx_gemm_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
-                   const MgParams p) {
+// Wide kernel, one cluster of two CTAs per tile in turn.  CTA r of the pair holds tokens
+// [128 r, +128) of the tile in its half of operand A, weight rows [128 r, +128) of the tile as its
+// half of operand B, and the scales of its tokens and of all the weight rows.  Its producer
+// fills its own shared memory and counts on the leader's full barrier; the leader issues the
+// scale copies and MMAs for both, and commits release the stage, or hand over the accumulator, in
+// both.  tmT, tmW: rows [*, cols_p/2] of the tokens and weights, box 128 B x 128; tmSfT, tmSfW: their
+// scale atoms as [*, 256] bytes, box 256 x 4 (two atoms).
+template <bool OUT32, bool SWIGLU>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape::THREADS, 1)
+    mx_wide_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ CUtensorMap tmSfT, const __grid_constant__ CUtensorMap tmSfW,
+                   const __grid_constant__ MgParams p) {
   pdl_wait();
   pdl_trigger();
-  using S = MgShape<FLAT, BN>;
+  using S = WideShape;
+  constexpr int STAGES = S::STAGES, EPW = S::EPW, COPIER = 2 + EPW;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = sA + STAGES * MG_A_BYTES;
+  uint8_t* sSFA = sB + STAGES * S::B_BYTES;
+  uint8_t* sSFB = sSFA + STAGES * MG_SF_BYTES;
+  uint8_t* sSTG = sSFB + STAGES * 2 * MG_SF_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);   // the leader's are used
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* sff_bar = empty_bar + STAGES;          // the stage's scales are in TMEM (the leader's)
+  uint64_t* tfull_bar = sff_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 1;            // the leader's
+  uint64_t* drain_bar = tempty_bar + 1;            // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
+  static_assert((3 * STAGES + 4) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t crank = cluster_ctarank();
+  const bool leader = crank == 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+      mbar_init(smem_u32(&sff_bar[s]), 1);
+    }
+    mbar_init(smem_u32(tfull_bar), 1);
+    mbar_init(smem_u32(tempty_bar), 2 * EPW);
+    mbar_init(smem_u32(&drain_bar[0]), 1);
+    mbar_init(smem_u32(&drain_bar[1]), 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tmT);
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmSfT);
+    tma_prefetch_desc(&tmSfW);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), MG_TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();                                  // barriers set up and TMEM allocated in both CTAs
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int n_tiles = p.n_tiles ? min(*p.n_tiles, p.max_tiles) : p.max_tiles;
+  const int total = n_tiles * p.n_wt;
+  const int n_kblk = (int)((p.katoms + 1) / 2);
+  const int t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const uint64_t timeout = p.timeout_ns ? p.timeout_ns : 2000000000ull;
+
+  if (warp == 0) {
+    // ───────── producer (both CTAs) ─────────
+    int stage = 0;
+    uint32_t phase = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    const int wblk = (p.N + 127) / 128;
+    for (int t = t0; ok && t < total; t += step) {
+      const int tt = t / p.n_wt, wt = t % p.n_wt;
+      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const int trow = (int)tile.row0 + (int)crank * 128;
+      const int wrow = tile.e * p.N + wt * 256 + (int)crank * 128;
+      const int sft = (int)((tile.slot * 2 + crank) * p.katoms * 2);           // rows of 256 B: two an atom
+      const int sfw = (int)(((int64_t)tile.e * wblk + wt * 2) * p.katoms * 2);
+      for (int kb = 0; kb < n_kblk; ++kb) {
+        if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          const uint32_t fb_local = smem_u32(&full_bar[stage]);
+          const uint32_t fb = mapa_shared(fb_local, 0);
+          if (leader) mbar_arrive_expect_tx(fb_local, 2u * S::STAGE);
+          tma_load_2d_pair(smem_u32(sA + stage * MG_A_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
+          tma_load_2d_pair(smem_u32(sB + stage * S::B_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
+          // (at the end of an odd row of atoms the second atom is the next block's: not used)
+          tma_load_2d_pair(smem_u32(sSFA + stage * MG_SF_BYTES), &tmSfT, fb, 0, sft + kb * 4);
+          const uint32_t sb = smem_u32(sSFB + stage * 2 * MG_SF_BYTES);
+          tma_load_2d_pair(sb, &tmSfW, fb, 0, sfw + kb * 4);
+          tma_load_2d_pair(sb + MG_SF_BYTES, &tmSfW, fb, 0, sfw + (int)p.katoms * 2 + kb * 4);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    // The leader's full barriers count both CTAs' bytes: with the last of them every copy has landed.
+    if (leader)
+      for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+        mbar_wait(smem_u32(&full_bar[i % STAGES]), (uint32_t)((i / STAGES) & 1), nullptr, 0, MHMOE_DRAIN_NS);
+  } else if (warp == 1) {
+    // ───────── MMA issuer (leader) ─────────
+    if (leader) {
+      int stage = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      constexpr uint32_t idesc[2] = {idesc_mxf4(2 * MG_BM, 256, 0), idesc_mxf4(2 * MG_BM, 256, 2)};
+      for (int t = t0; t < total; t += step) {
+        if (!mbar_wait(smem_u32(tempty_bar), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+        tc_fence_after();
+        for (int kb = 0; kb < n_kblk; ++kb) {
+          if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+          if (!mbar_wait(smem_u32(&sff_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
+            const uint32_t a_s = smem_u32(sA + stage * MG_A_BYTES);
+            const uint32_t b_s = smem_u32(sB + stage * S::B_BYTES);
+            const int nj = (int)min(4u, 2 * (p.katoms - 2 * kb));    // 64-column steps of this stage
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (j < nj)
+                mma_mxf4_pair(tmem_base, sdesc_kmajor_sw128(a_s + j * 32), sdesc_kmajor_sw128(b_s + j * 32),
+                              idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 8, (kb | j) != 0 ? 1u : 0u);
+            }
+            const uint32_t eb = smem_u32(&empty_bar[stage]);
+            tc_commit_pair(mapa_shared(eb, 0));
+            tc_commit_pair(mapa_shared(eb, 1));
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (lane == 0) {
+          tc_commit_pair(mapa_shared(smem_u32(tfull_bar), 0));
+          tc_commit_pair(mapa_shared(smem_u32(tfull_bar), 1));
+        }
+        __syncwarp();
+        acc_phase ^= 1;
+      }
+    }
+  } else if (warp == COPIER) {
+    // ───────── scale copier (leader) ─────────
+    // Slot s is rewritten only after full[s] of the next round, posted after empty[s], which the
+    // MMA warp commits after the MMAs that read the slot.
+    if (leader) {
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int t = t0; t < total; t += step) {
+        for (int kb = 0; kb < n_kblk; ++kb) {
+          if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
+            const uint32_t sa = smem_u32(sSFA + stage * MG_SF_BYTES), sb = smem_u32(sSFB + stage * 2 * MG_SF_BYTES);
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              tc_cp_32x128b_warpx4_pair(tsfa + a * 4, sdesc_sf_chunk(sa + a * 512));
+              tc_cp_32x128b_warpx4_pair(tsfb + a * 8, sdesc_sf_chunk(sb + a * 512));
+              tc_cp_32x128b_warpx4_pair(tsfb + a * 8 + 4, sdesc_sf_chunk(sb + MG_SF_BYTES + a * 512));
+            }
+            tc_commit_pair(mapa_shared(smem_u32(&sff_bar[stage]), 0));
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+    }
+  } else {
+    // ───────── epilogue (both CTAs, their own 128 tokens) ─────────
+    const int q = warp & 3;                        // TMEM lane quarter of this warp
+    const int slice = (warp - 2) >> 2;             // accumulator columns [64 * slice, +64)
+    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty_bar), 0);
+    uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
+    uint32_t acc_phase = 0;
+    const int m0 = (int)crank * 128 + q * 32;
+    for (int t = t0; t < total; t += step) {
+      const int tt = t / p.n_wt, wt = t % p.n_wt;
+      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      if (!mbar_wait(smem_u32(tfull_bar), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
+      acc_phase ^= 1;
+      tc_fence_after();
+      uint32_t r[64];
+      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(slice * 64);
+      MHMOE_TMEM_LD_32x32b_X32(taddr, (r + 0));
+      MHMOE_TMEM_LD_32x32b_X32(taddr + 32, (r + 32));
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty_leader);
+      if (m0 < tile.rows) mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * 256 + slice * 64, m0, lane, stg);
+    }
+  }
+done:
+  // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
+  if (leader && warp == 1 && lane == 0) {
+    tc_commit_pair(mapa_shared(smem_u32(&drain_bar[0]), 0));
+    mbar_wait(smem_u32(&drain_bar[0]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+  }
+  if (leader && warp == COPIER && lane == 0) {
+    tc_commit_pair(mapa_shared(smem_u32(&drain_bar[1]), 0));
+    mbar_wait(smem_u32(&drain_bar[1]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+  }
+  tc_fence_before();
+  cluster_sync();                                  // neither CTA leaves while the pair still uses it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, MG_TMEM_COLS);
+  }
+}
+
+// Flat kernel.  tmT: token rows [R, cols_p/2], box 128 B x BN; tmW: weight rows [n * N, cols_p/2], box
+// 128 B x 128.  SPLIT: a cluster of CTAs shares one work item along the columns; their partial
+// accumulators meet in distributed shared memory and are summed in the order of the ranks.
+template <int BN, bool SPLIT, bool OUT32>
+__global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
+    mx_flat_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
+                   const __grid_constant__ MgParams p) {
+  pdl_wait();
+  pdl_trigger();
+  using S = FlatShape<BN>;
   constexpr int STAGES = S::STAGES, EPW = S::EPW, COPIER = 2 + EPW, NACC = S::NACC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = sA + STAGES * MG_A_BYTES;
   uint8_t* sSFA = sB + STAGES * S::B_BYTES;
-  uint8_t* sSFB = sSFA + STAGES * MG_SFA_BYTES;
-  uint8_t* sSTG = sSFB + STAGES * S::SFB_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + S::STG);
+  uint8_t* sSFB = sSFA + STAGES * MG_SF_BYTES;
+  uint8_t* sSTG = sSFB + STAGES * MG_SF_BYTES;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sff_bar = empty_bar + STAGES;      // the stage's scales are in TMEM
   uint64_t* tfull_bar = sff_bar + STAGES;      // [NACC]
@@ -224,6 +472,7 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
   uint64_t* drain_bar = tempty_bar + NACC;     // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
   static_assert((3 * STAGES + 2 * NACC + 2) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  static_assert(!SPLIT || BN * 128 * 4 <= STAGES * MG_A_BYTES, "partial sums lie over operand A's stages");
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -276,11 +525,9 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
     for (int64_t t = t0; ok && t < total; t += step) {
       const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
       const MgTile tile = mg_tile<S::SLOT>(p, tt);
-      const int wrow = tile.e * p.N + wt * S::WROWS;
-      const uint32_t wb = wt * (S::WROWS / 128);
+      const int wrow = tile.e * p.N + wt * 128;
       const uint8_t* sf_t = p.sf_tok + (uint64_t)tile.slot * p.katoms * 512;
-      const uint8_t* sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wb) * p.katoms * 512;
-      const bool second = S::WROWS == 256 && wb + 1 < wblk;       // the weight tile's second atom block exists
+      const uint8_t* sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wt) * p.katoms * 512;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) {
           ok = false;
@@ -289,14 +536,11 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
         if (lane == 0) {
           const uint32_t fb = smem_u32(&full_bar[stage]);
           const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;  // atoms of this stage
-          mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * (2 + (second ? 1 : 0)));
-          const uint32_t a = smem_u32(sA + stage * MG_A_BYTES), b = smem_u32(sB + stage * S::B_BYTES);
-          const uint32_t sa = smem_u32(sSFA + stage * MG_SFA_BYTES), sb = smem_u32(sSFB + stage * S::SFB_BYTES);
-          tma_load_2d(FLAT ? b : a, &tmT, fb, kb * (MG_BK / 2), (int)tile.row0);
-          tma_load_2d(FLAT ? a : b, &tmW, fb, kb * (MG_BK / 2), wrow);
-          bulk_load(FLAT ? sb : sa, sf_t + kb * 1024, sfn, fb);
-          bulk_load(FLAT ? sa : sb, sf_w + kb * 1024, sfn, fb);
-          if (second) bulk_load(sb + MG_SFA_BYTES, sf_w + (uint64_t)p.katoms * 512 + kb * 1024, sfn, fb);
+          mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * 2);
+          tma_load_2d(smem_u32(sA + stage * MG_A_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
+          tma_load_2d(smem_u32(sB + stage * S::B_BYTES), &tmT, fb, kb * (MG_BK / 2), (int)tile.row0);
+          bulk_load(smem_u32(sSFA + stage * MG_SF_BYTES), sf_w + kb * 1024, sfn, fb);
+          bulk_load(smem_u32(sSFB + stage * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
         }
         __syncwarp();
         ++issued;
@@ -327,8 +571,7 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
           for (int j = 0; j < 4; ++j) {
             if (j < nj)
               mma_mxf4(tmem_base + acc * BN, sdesc_kmajor_sw128(a_s + j * 32), sdesc_kmajor_sw128(b_s + j * 32),
-                       idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 4 * S::NBLK,
-                       (kb > kb0 || j > 0) ? 1u : 0u);
+                       idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 4, (kb > kb0 || j > 0) ? 1u : 0u);
           }
           tc_commit(smem_u32(&empty_bar[stage]));
         }
@@ -349,14 +592,12 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
         tc_fence_after();
         if (lane == 0) {
           const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
-          const uint32_t sa = smem_u32(sSFA + stage * MG_SFA_BYTES), sb = smem_u32(sSFB + stage * S::SFB_BYTES);
+          const uint32_t sa = smem_u32(sSFA + stage * MG_SF_BYTES), sb = smem_u32(sSFB + stage * MG_SF_BYTES);
 #pragma unroll
           for (int a = 0; a < 2; ++a) {
             if (2 * kb + a < (int)p.katoms) {
               tc_cp_32x128b_warpx4(tsfa + a * 4, sdesc_sf_chunk(sa + a * 512));
-#pragma unroll
-              for (int b = 0; b < S::NBLK; ++b)
-                tc_cp_32x128b_warpx4(tsfb + (a * S::NBLK + b) * 4, sdesc_sf_chunk(sb + b * MG_SFA_BYTES + a * 512));
+              tc_cp_32x128b_warpx4(tsfb + a * 4, sdesc_sf_chunk(sb + a * 512));
             }
           }
           tc_commit(smem_u32(&sff_bar[stage]));
@@ -368,47 +609,36 @@ __global__ void __launch_bounds__(MgShape<FLAT, BN>::THREADS, 1)
   } else {
     // ───────── epilogue ─────────
     const int q = warp & 3;                    // TMEM lane quarter of this warp
+    const int part = (warp - 2) >> 2;          // with 8 warps: every other chunk of columns
+    constexpr int NC = BN < 32 ? BN : 32;
+    uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t t = t0; t < total; t += step) {
       const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
       const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const int n0 = wt * 128 + q * 32;
+      const float b = p.bias && n0 + lane < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n0 + lane) : 0.f;
       if (!mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
       tc_fence_after();
       const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
-      if constexpr (!FLAT) {
-        const int half = (warp - 2) >> 2;      // accumulator columns [128 * half, +128)
-        uint32_t r[128];
-#pragma unroll
-        for (int c = 0; c < 128; c += 32) MHMOE_TMEM_LD_32x32b_X32(taddr + half * 128 + c, (r + c));
+      for (int j0 = part * NC; j0 < BN && j0 < tile.rows; j0 += NC * (EPW / 4)) {
+        uint32_t r[NC];
+        if constexpr (NC == 16) MHMOE_TMEM_LD_32x32b_X16(taddr + j0, r);
+        else MHMOE_TMEM_LD_32x32b_X32(taddr + j0, r);
         tmem_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
-        if (q * 32 < tile.rows)
-          mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * 256 + half * 128, q, lane, sSTG + (warp - 2) * MG_STG_BYTES);
-      } else {
-        const int n = wt * 128 + q * 32 + lane;
-        const float b = p.bias && n < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n) : 0.f;
-        constexpr int NC = BN < 32 ? BN : 32;
-        for (int j0 = 0; j0 < BN && j0 < tile.rows; j0 += NC) {
-          uint32_t r[NC];
-          if constexpr (NC == 16) MHMOE_TMEM_LD_32x32b_X16(taddr + j0, r);
-          else MHMOE_TMEM_LD_32x32b_X32(taddr + j0, r);
-          tmem_wait_ld();
-          if constexpr (SPLIT) {
-            // partial sums [token][weight row] over the stages' memory, all of it consumed by now
-            float* red = reinterpret_cast<float*>(smem);
+        if constexpr (SPLIT) {
+          // partial sums [token][weight row] over the stages' memory, all of it consumed by now
+          float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
-            for (int j = 0; j < NC; ++j) red[(j0 + j) * 128 + q * 32 + lane] = __uint_as_float(r[j]);
-          } else {
-            mg_flat_columns<NC>(p, tile, r, j0, n, b);
-          }
+          for (int j = 0; j < NC; ++j) red[(j0 + j) * 128 + q * 32 + lane] = __uint_as_float(r[j]);
+        } else {
+          if (n0 < p.N) mg_flat_epilogue<NC, OUT32>(p, tile, r, j0, n0, b, lane, stg);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&tempty_bar[acc]));
       if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
     }
   }
@@ -578,7 +808,8 @@ __global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>
   if (!ok && lane == 0) record_error(p.status, MHMOE_ERR_ARGS);
   const typename MxType<DT>::T* xr = x + (ok ? src : 0) * p.x_stride;
   uint8_t* d = p.data + r * (int64_t)p.katoms * 64;
-  uint8_t* s = p.sf + (uint64_t)slot * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
+  const int blocks = (p.slot_rows + 127) / 128;
+  uint8_t* s = p.sf + ((uint64_t)slot * blocks + (m >> 7)) * p.katoms * 512 + (m & 31) * 16 + ((m >> 5) & 3) * 4;
 #pragma unroll 2
   for (uint32_t c0 = lane * 16; c0 < (p.katoms + 3) / 4 * 512; c0 += 512) {
     MxRaw16<typename MxType<DT>::T> v;
@@ -616,10 +847,10 @@ MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
     g.flat = true;
     g.bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   } else {
-    g.flat = tiles_of(128) * ceil_div(N, 256) < sms;
-    g.bn = g.flat ? 128 : 256;
+    g.flat = tiles_of(256) * ceil_div(N, 256) < sms / 2;
+    g.bn = 128;
   }
-  g.slot_rows = g.flat ? g.bn : 128;
+  g.slot_rows = g.flat ? g.bn : 256;
   g.tiles = tiles_of(g.slot_rows);
   g.slots = grouped ? R / g.slot_rows + n + 1 : g.tiles;
   g.n_wt = (int)ceil_div(N, g.flat ? 128 : 256);
@@ -637,17 +868,44 @@ MgScratch mg_scratch(const MgPlan& g, int64_t R, int64_t katoms, bool grouped) {
   MgScratch s;
   s.data = 0;
   s.sf = up((size_t)R * katoms * 64);
-  s.tiles = s.sf + up((size_t)(grouped ? g.slots : ceil_div(R, 128)) * katoms * 512);
+  const int64_t blocks = grouped ? g.slots * ceil_div(g.slot_rows, 128) : ceil_div(R, 128);
+  s.tiles = s.sf + up((size_t)blocks * katoms * 512);
   s.count = s.tiles + (grouped ? up((size_t)g.tiles * sizeof(int4)) : 0);
   s.bytes = s.count + (grouped ? 256 : 0);
   return s;
 }
 
-template <bool FLAT, int BN, bool SPLIT, bool OUT32, bool SWIGLU>
-cudaError_t mg_launch(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
-                      cudaStream_t st) {
-  using S = MgShape<FLAT, BN>;
-  auto kernel = mx_gemm_kernel<FLAT, BN, SPLIT, OUT32, SWIGLU>;
+template <bool OUT32, bool SWIGLU>
+cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const CUtensorMap& tsft, const CUtensorMap& tsfw,
+                        const MgParams& p, const MgPlan& g, cudaStream_t st) {
+  using S = WideShape;
+  auto kernel = mx_wide_kernel<OUT32, SWIGLU>;
+  // per device: the shared-memory attribute and the clusters that fit at once
+  static PerDeviceOnce once;
+  static int max_clusters[MHMOE_MAX_DEVICES] = {};
+  const cudaError_t attr = once.run([&](int dev) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * (num_sms() / 2));
+    cfg.blockDim = dim3(S::THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    e = cudaOccupancyMaxActiveClusters(&max_clusters[dev], kernel, &cfg);
+    if (e == cudaSuccess && max_clusters[dev] <= 0) e = cudaErrorInvalidConfiguration;
+    return e;
+  });
+  if (attr != cudaSuccess) return attr;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const int64_t clusters = std::min<int64_t>(max_clusters[dev], g.tiles * g.n_wt);
+  return launch_pdl(kernel, dim3((unsigned)(2 * clusters)), dim3(S::THREADS), S::SMEM, st, tt, tw, tsft, tsfw, p);
+}
+
+template <int BN, bool SPLIT, bool OUT32>
+cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                        cudaStream_t st) {
+  using S = FlatShape<BN>;
+  auto kernel = mx_flat_kernel<BN, SPLIT, OUT32>;
   static PerDeviceOnce once;
   const cudaError_t attr = once.run(
       [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
@@ -676,10 +934,11 @@ cudaError_t mg_launch(const CUtensorMap& tt, const CUtensorMap& tw, const MgPara
 }
 
 template <int BN>
-cudaError_t mg_launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
-                           cudaStream_t st) {
-  return g.split > 1 ? mg_launch<true, BN, true, false, false>(tt, tw, p, g, st)
-                     : mg_launch<true, BN, false, false, false>(tt, tw, p, g, st);
+cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                        cudaStream_t st) {
+  if (g.split > 1) return launch_flat<BN, true, false>(tt, tw, p, g, st);
+  return p.y_dtype == DT_F32 ? launch_flat<BN, false, true>(tt, tw, p, g, st)
+                             : launch_flat<BN, false, false>(tt, tw, p, g, st);
 }
 
 }  // namespace
@@ -758,20 +1017,29 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
   a.status = p.status;
   a.timeout_ns = p.timeout_ns;
   CUtensorMap tt, tw;
-  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)g.slot_rows) != cudaSuccess ||
-      encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, g.flat ? 128 : 256) != cudaSuccess)
+  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)std::min(g.slot_rows, 128)) !=
+          cudaSuccess ||
+      encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, 128) != cudaSuccess)
     return MHMOE_ERR_DRIVER;
   if (g.flat) {
-    *cerr = g.bn == 16   ? mg_launch_flat<16>(tt, tw, a, g, st)
-            : g.bn == 32 ? mg_launch_flat<32>(tt, tw, a, g, st)
-            : g.bn == 64 ? mg_launch_flat<64>(tt, tw, a, g, st)
-                         : mg_launch_flat<128>(tt, tw, a, g, st);
-  } else if (p.y_dtype == DT_F32) {
-    *cerr = p.act ? mg_launch<false, 256, false, true, true>(tt, tw, a, g, st)
-                  : mg_launch<false, 256, false, true, false>(tt, tw, a, g, st);
+    *cerr = g.bn == 16   ? launch_flat<16>(tt, tw, a, g, st)
+            : g.bn == 32 ? launch_flat<32>(tt, tw, a, g, st)
+            : g.bn == 64 ? launch_flat<64>(tt, tw, a, g, st)
+                         : launch_flat<128>(tt, tw, a, g, st);
   } else {
-    *cerr = p.act ? mg_launch<false, 256, false, false, true>(tt, tw, a, g, st)
-                  : mg_launch<false, 256, false, false, false>(tt, tw, a, g, st);
+    const int64_t blocks = grouped ? g.slots * 2 : ceil_div(p.R, 128), wblk = ceil_div(p.N, 128);
+    CUtensorMap tsft, tsfw;
+    if (encode_tmap_2d(&tsft, a.sf_tok, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 256, (uint64_t)blocks * katoms * 2, 256, 256, 4,
+                       false) != cudaSuccess ||
+        encode_tmap_2d(&tsfw, p.w_sf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 256, (uint64_t)p.n * wblk * katoms * 2, 256, 256,
+                       4, false) != cudaSuccess)
+      return MHMOE_ERR_DRIVER;
+    if (p.y_dtype == DT_F32)
+      *cerr = p.act ? launch_wide<true, true>(tt, tw, tsft, tsfw, a, g, st)
+                    : launch_wide<true, false>(tt, tw, tsft, tsfw, a, g, st);
+    else
+      *cerr = p.act ? launch_wide<false, true>(tt, tw, tsft, tsfw, a, g, st)
+                    : launch_wide<false, false>(tt, tw, tsft, tsfw, a, g, st);
   }
   return *cerr == cudaSuccess ? MHMOE_OK : MHMOE_ERR_LAUNCH;
 }
