@@ -9,9 +9,7 @@
 // (tcgen05.mma kind::mxf4, fp32 accumulators in TMEM).
 //
 // A work item is (token tile, weight tile), in one of two kernels:
-//   wide   256 tokens x 256 weight rows on a pair of CTAs (cta_group::2): 128 tokens a CTA, each
-//          loads half of the weight rows.  One CTA alone would read 51 KB a stage (256 columns)
-//          through a 64 B/clk port, 800 clocks for 549 of MMA; the pair reads 35 KB each.
+//   wide   128 tokens x 256 weight rows: the most math per operand byte
 //   flat   128 weight rows x 16..128 tokens: with a few tokens the instruction's 128 lanes are
 //          filled by the weights, which is what a decode step streams.  A cluster may share an
 //          item along the columns.
@@ -27,15 +25,15 @@ constexpr int MG_BM = 128;                  // rows of operand A a CTA
 constexpr int MG_BK = 256;                  // columns of a stage: 128 B a row
 constexpr int MG_A_BYTES = MG_BM * MG_BK / 2;
 constexpr int MG_SF_BYTES = 2 * 512;        // scales of 128 rows x 256 columns: two atoms
-constexpr int MG_STG_BYTES = 2048;          // store staging per epilogue warp: 32 rows x 64 B
+constexpr int MG_STG_BYTES = 1024;          // store staging per epilogue warp: 32 rows x 32 B
 constexpr int MG_MISC_BYTES = 512;          // barriers, TMEM slot
 constexpr int MG_TMEM_COLS = 512;
 
 struct WideShape {
-  static constexpr int SLOT = 256, WROWS = 256;                 // tokens and weight rows of a tile
-  static constexpr int B_BYTES = MG_BM * MG_BK / 2;             // half of the weight rows
+  static constexpr int SLOT = 128, BN = 256;                    // tokens and weight rows of a tile
+  static constexpr int B_BYTES = BN * MG_BK / 2;
   static constexpr int STAGE = MG_A_BYTES + B_BYTES + 3 * MG_SF_BYTES;
-  static constexpr int STAGES = 5;
+  static constexpr int STAGES = 4;
   static constexpr int EPW = 16;                                // epilogue warps: 64 columns each
   static constexpr int THREADS = 32 * (3 + EPW);
   static constexpr int SMEM = STAGES * STAGE + EPW * MG_STG_BYTES + MG_MISC_BYTES + 1024;
@@ -46,7 +44,7 @@ struct WideShape {
 
 template <int BN>
 struct FlatShape {
-  static constexpr int SLOT = BN, WROWS = MG_BM;
+  static constexpr int SLOT = BN;                               // tokens of a tile
   static constexpr int B_BYTES = BN * MG_BK / 2;
   static constexpr int STAGE = MG_A_BYTES + B_BYTES + 2 * MG_SF_BYTES;
   static constexpr int EPW = BN >= 64 ? 8 : 4;
@@ -60,7 +58,7 @@ struct FlatShape {
 };
 
 struct MgParams {
-  const uint8_t* sf_tok;      // scale atoms of the token tiles, ceil(SLOT / 128) blocks of 128 rows per slot
+  const uint8_t* sf_tok;      // scale atoms of the token tiles, a 128-row block per slot
   const uint8_t* sf_w;
   const int4* tiles;          // grouped: {expert, first row, rows, slot}; null: dense
   const int* n_tiles;         // grouped: their number (device)
@@ -117,26 +115,29 @@ __device__ __forceinline__ void mg_store(void* y, int dtype, int64_t at, float v
   else static_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-// 32 rows x 64 B of the warp's staging (16-B chunks xor-swizzled over row pairs) to the rows
-// row0 + 0.. of y, `rows` of them, from output column c0; `width` outputs a row are valid.
+// Byte offset of 16-B chunk k (0, 1) of a staging row of 32 B: four rows fill the 32 banks once.
+__device__ __forceinline__ int mg_stg(int row, int k) { return row * 32 + ((k ^ ((row >> 2) & 1)) << 4); }
+
+// 32 rows x 32 B of the warp's staging to the rows row0 + 0.. of y, `rows` of them, from output
+// column c0; `width` outputs a row are valid.
 template <int ESZ>
 __device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* stg, int64_t row0, int rows, int c0,
                                               int width, int lane) {
   uint8_t* y = static_cast<uint8_t*>(p.y);
   if (p.y_vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = i * 8 + (lane >> 2), k = lane & 3;
+    for (int i = 0; i < 2; ++i) {
+      const int row = i * 16 + (lane >> 1), k = lane & 1;
       if (row < rows && k * (16 / ESZ) < width)
         *reinterpret_cast<uint4*>(y + ((row0 + row) * p.y_stride + c0 + k * (16 / ESZ)) * ESZ) =
-            *reinterpret_cast<const uint4*>(stg + row * 64 + ((k ^ ((row >> 1) & 3)) << 4));
+            *reinterpret_cast<const uint4*>(stg + mg_stg(row, k));
     }
   } else {
-    constexpr int PER = 64 / ESZ;                   // one output a lane, two rows at once in fp32
+    constexpr int PER = 32 / ESZ;                   // one output a lane
     const int col = lane % PER;
     for (int row = lane / PER; row < rows; row += 32 / PER) {
       if (col >= width) break;
-      const uint8_t* src = stg + row * 64 + (((col * ESZ >> 4) ^ ((row >> 1) & 3)) << 4) + (col * ESZ & 15);
+      const uint8_t* src = stg + mg_stg(row, col * ESZ >> 4) + (col * ESZ & 15);
       uint8_t* dst = y + ((row0 + row) * p.y_stride + c0 + col) * ESZ;
       if constexpr (ESZ == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
       else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
@@ -148,7 +149,7 @@ __device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* 
 template <bool OUT32, bool SWIGLU>
 __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, uint32_t (&r)[64], int col0,
                                                  int m0, int lane, uint8_t* stg) {
-  constexpr int PER = OUT32 ? 16 : 32;              // outputs of a 64-B chunk
+  constexpr int PER = OUT32 ? 8 : 16;               // outputs of a 32-B chunk
   constexpr int ACC = SWIGLU ? 2 * PER : PER;       // accumulator columns behind them
   const int n_out = SWIGLU ? p.N / 2 : p.N;
   if (p.bias) {
@@ -176,14 +177,14 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
     }
     __syncwarp();                                   // the chunk before has left the staging
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < 2; ++k) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (OUT32) w[j] = __float_as_uint(v[4 * k + j]);
         else w[j] = mg_pack16(v[8 * k + 2 * j], v[8 * k + 2 * j + 1], half);
       }
-      *reinterpret_cast<uint4*>(stg + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(stg + mg_stg(lane, k)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
     const int o0 = SWIGLU ? (col0 + c * ACC) / 2 : col0 + c * ACC;
@@ -192,12 +193,12 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
 }
 
 // Flat epilogue: one weight row n a thread (32 of the warp's from n0) x NC token columns from j0.
-// The transposed outputs go through the staging in passes of 64 B a token row.
+// The transposed outputs go through the staging in passes of 32 B a token row.
 template <int NC, bool OUT32>
 __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile& t, const uint32_t (&r)[NC], int j0,
                                                  int n0, float b, int lane, uint8_t* stg) {
   using U = typename std::conditional<OUT32, float, uint16_t>::type;
-  constexpr int ESZ = OUT32 ? 4 : 2, PER = 64 / ESZ;
+  constexpr int ESZ = OUT32 ? 4 : 2, PER = 32 / ESZ;
   const bool half = p.y_dtype == DT_F16;
   const int rows = min(NC, t.rows - j0);
   // a row's weight, from the lane that holds it
@@ -213,14 +214,14 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
   const int n_out = p.act ? p.N / 2 : p.N, o0 = p.act ? n0 / 2 : n0;
   const int width = p.act ? 16 : 32;                // outputs of the warp a token row
 #pragma unroll
-  for (int c = 0; c < 32 / PER; ++c) {              // fp32 without activation: two passes of 16 outputs
+  for (int c = 0; c < 32 / PER; ++c) {
     if (c * PER >= width) break;
     const int at = (p.act ? lane >> 1 : lane) - c * PER;
     __syncwarp();
     if (at >= 0 && at < PER && !(p.act && (lane & 1))) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        U* dst = reinterpret_cast<U*>(stg + j * 64 + (((at * ESZ >> 4) ^ ((j >> 1) & 3)) << 4) + (at * ESZ & 15));
+        U* dst = reinterpret_cast<U*>(stg + mg_stg(j, at * ESZ >> 4) + (at * ESZ & 15));
         if constexpr (OUT32) *dst = v[j];
         else *dst = (uint16_t)mg_pack16(v[j], 0.f, half);
       }
@@ -230,17 +231,40 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
   }
 }
 
-// Wide kernel, one cluster of two CTAs per tile in turn.  CTA r of the pair holds tokens
-// [128 r, +128) of the tile in its half of operand A, weight rows [128 r, +128) of the tile as its
-// half of operand B, and the scales of its tokens and of all the weight rows.  Its producer
-// fills its own shared memory and counts on the leader's full barrier; the leader issues the
-// scale copies and MMAs for both, and commits release the stage, or hand over the accumulator, in
-// both.  tmT, tmW: rows [*, cols_p/2] of the tokens and weights, box 128 B x 128; tmSfT, tmSfW: their
-// scale atoms as [*, 256] bytes, box 256 x 4 (two atoms).
+// The producer, copier and MMA warps share their schedulers with busy epilogue warps, so every
+// instruction of theirs between two asynchronous operations costs tensor time (a loop over the
+// stages with descriptors made on the way ran 803 clocks a stage of 8192^2 x 4096, this form 700).
+// Hence: the stages are unrolled, so that barriers, descriptors and TMEM columns are constants
+// plus a base; the elected lane and the role are warp-uniform values; all 512 TMEM columns are
+// allocated, so addresses start at 0; and each role reads its next tile's entry a tile ahead.
+//
+// role(t, kb, s, phase): one stage of item t in ring slot s.  Items t0, t0 + step, ... below total, stages
+// kb0 .. kb1 of each; ends where a call returns false.  UNROLL: slots are constants (the flat
+// kernel, whose 5 to 9 slots of four roles would not fit the instruction cache, streams weights
+// and does without: 27 against 34 us for 32 tokens over 128 experts).
+template <int STAGES, bool UNROLL, class Stage>
+__device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int kb0, int kb1, Stage&& role) {
+  int t = t0, kb = kb0;
+  uint32_t phase = 0;
+  while (t < total) {
+#pragma unroll(UNROLL ? STAGES : 1)
+    for (int s = 0; s < STAGES; ++s) {
+      if (!role(t, kb, s, phase)) return;
+      if (++kb == kb1) {
+        kb = kb0;
+        t += step;
+        if (t >= total) return;
+      }
+    }
+    phase ^= 1;
+  }
+}
+
+// Wide kernel.  tmT: token rows [R, cols_p/2], box 128 B x 128; tmW: weight rows [n * N, cols_p/2], box
+// 128 B x 256.
 template <bool OUT32, bool SWIGLU>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape::THREADS, 1)
+__global__ void __launch_bounds__(WideShape::THREADS, 1)
     mx_wide_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
-                   const __grid_constant__ CUtensorMap tmSfT, const __grid_constant__ CUtensorMap tmSfW,
                    const __grid_constant__ MgParams p) {
   pdl_wait();
   pdl_trigger();
@@ -253,19 +277,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape::THREADS, 
   uint8_t* sSFA = sB + STAGES * S::B_BYTES;
   uint8_t* sSFB = sSFA + STAGES * MG_SF_BYTES;
   uint8_t* sSTG = sSFB + STAGES * 2 * MG_SF_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);   // the leader's are used
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* sff_bar = empty_bar + STAGES;          // the stage's scales are in TMEM (the leader's)
+  uint64_t* sff_bar = empty_bar + STAGES;          // the stage's scales are in TMEM
   uint64_t* tfull_bar = sff_bar + STAGES;
-  uint64_t* tempty_bar = tfull_bar + 1;            // the leader's
+  uint64_t* tempty_bar = tfull_bar + 1;
   uint64_t* drain_bar = tempty_bar + 1;            // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
   static_assert((3 * STAGES + 4) * 8 + 4 <= MG_MISC_BYTES, "barriers");
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
   const int lane = threadIdx.x & 31;
-  const uint32_t crank = cluster_ctarank();
-  const bool leader = crank == 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
@@ -273,176 +295,157 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(WideShape::THREADS, 
       mbar_init(smem_u32(&sff_bar[s]), 1);
     }
     mbar_init(smem_u32(tfull_bar), 1);
-    mbar_init(smem_u32(tempty_bar), 2 * EPW);
+    mbar_init(smem_u32(tempty_bar), EPW);
     mbar_init(smem_u32(&drain_bar[0]), 1);
     mbar_init(smem_u32(&drain_bar[1]), 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmSfT);
-    tma_prefetch_desc(&tmSfW);
   }
   if (warp == 1) {
-    tmem_alloc_pair(smem_u32(tmem_slot), MG_TMEM_COLS);
-    tmem_relinquish_pair();
+    tmem_alloc(smem_u32(tmem_slot), MG_TMEM_COLS);
+    tmem_relinquish();
   }
   tc_fence_before();
-  cluster_sync();                                  // barriers set up and TMEM allocated in both CTAs
+  __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
 
   const int n_tiles = p.n_tiles ? min(*p.n_tiles, p.max_tiles) : p.max_tiles;
   const int total = n_tiles * p.n_wt;
   const int n_kblk = (int)((p.katoms + 1) / 2);
-  const int t0 = blockIdx.x >> 1, step = gridDim.x >> 1;
+  const int t0 = blockIdx.x, step = gridDim.x;
   const uint64_t timeout = p.timeout_ns ? p.timeout_ns : 2000000000ull;
 
   if (warp == 0) {
-    // ───────── producer (both CTAs) ─────────
-    int stage = 0;
-    uint32_t phase = 0;
+    // ───────── producer ─────────
+    const bool one = elect_one();
     int64_t issued = 0;
-    bool ok = true;
-    const int wblk = (p.N + 127) / 128;
-    for (int t = t0; ok && t < total; t += step) {
-      const int tt = t / p.n_wt, wt = t % p.n_wt;
-      const MgTile tile = mg_tile<S::SLOT>(p, tt);
-      const int trow = (int)tile.row0 + (int)crank * 128;
-      const int wrow = tile.e * p.N + wt * 256 + (int)crank * 128;
-      const int sft = (int)((tile.slot * 2 + crank) * p.katoms * 2);           // rows of 256 B: two an atom
-      const int sfw = (int)(((int64_t)tile.e * wblk + wt * 2) * p.katoms * 2);
-      for (int kb = 0; kb < n_kblk; ++kb) {
-        if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          const uint32_t fb_local = smem_u32(&full_bar[stage]);
-          const uint32_t fb = mapa_shared(fb_local, 0);
-          if (leader) mbar_arrive_expect_tx(fb_local, 2u * S::STAGE);
-          tma_load_2d_pair(smem_u32(sA + stage * MG_A_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
-          tma_load_2d_pair(smem_u32(sB + stage * S::B_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
-          // (at the end of an odd row of atoms the second atom is the next block's: not used)
-          tma_load_2d_pair(smem_u32(sSFA + stage * MG_SF_BYTES), &tmSfT, fb, 0, sft + kb * 4);
-          const uint32_t sb = smem_u32(sSFB + stage * 2 * MG_SF_BYTES);
-          tma_load_2d_pair(sb, &tmSfW, fb, 0, sfw + kb * 4);
-          tma_load_2d_pair(sb + MG_SF_BYTES, &tmSfW, fb, 0, sfw + (int)p.katoms * 2 + kb * 4);
-        }
-        __syncwarp();
-        ++issued;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    const uint32_t wblk = (uint32_t)((p.N + 127) / 128);
+    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int trow = 0, wrow = 0;
+    const uint8_t *sf_t = nullptr, *sf_w = nullptr;
+    bool second = false;                                            // the weight tile's second atom block exists
+    mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int t, int kb, int s, uint32_t phase) {
+      if (kb == 0) {
+        const int wt = t % p.n_wt;
+        trow = (int)next.row0;
+        wrow = next.e * p.N + wt * S::BN;
+        sf_t = p.sf_tok + (uint64_t)next.slot * p.katoms * 512;
+        sf_w = p.sf_w + ((uint64_t)next.e * wblk + wt * 2) * p.katoms * 512;
+        second = wt * 2 + 1 < (int)wblk;
+        if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
       }
-    }
-    // The leader's full barriers count both CTAs' bytes: with the last of them every copy has landed.
-    if (leader)
-      for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
-        mbar_wait(smem_u32(&full_bar[i % STAGES]), (uint32_t)((i / STAGES) & 1), nullptr, 0, MHMOE_DRAIN_NS);
+      if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (one) {
+        const uint32_t fb = smem_u32(&full_bar[s]);
+        const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;      // atoms of this stage
+        mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * (2 + (second ? 1 : 0)));
+        tma_load_2d(smem_u32(sA + s * MG_A_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
+        tma_load_2d(smem_u32(sB + s * S::B_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
+        const uint32_t sb = smem_u32(sSFB + s * 2 * MG_SF_BYTES);
+        bulk_load(smem_u32(sSFA + s * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
+        bulk_load(sb, sf_w + kb * 1024, sfn, fb);
+        if (second) bulk_load(sb + MG_SF_BYTES, sf_w + (uint64_t)p.katoms * 512 + kb * 1024, sfn, fb);
+      }
+      __syncwarp();
+      ++issued;
+      return true;
+    });
+    // every copy lands before the CTA can exit (returns at once unless a consumer gave up)
+    for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
+      mbar_wait(smem_u32(&full_bar[i % STAGES]), (uint32_t)((i / STAGES) & 1), nullptr, 0, MHMOE_DRAIN_NS);
   } else if (warp == 1) {
-    // ───────── MMA issuer (leader) ─────────
-    if (leader) {
-      int stage = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      constexpr uint32_t idesc[2] = {idesc_mxf4(2 * MG_BM, 256, 0), idesc_mxf4(2 * MG_BM, 256, 2)};
-      for (int t = t0; t < total; t += step) {
-        if (!mbar_wait(smem_u32(tempty_bar), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-        tc_fence_after();
-        for (int kb = 0; kb < n_kblk; ++kb) {
-          if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-          if (!mbar_wait(smem_u32(&sff_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
-            const uint32_t a_s = smem_u32(sA + stage * MG_A_BYTES);
-            const uint32_t b_s = smem_u32(sB + stage * S::B_BYTES);
-            const int nj = (int)min(4u, 2 * (p.katoms - 2 * kb));    // 64-column steps of this stage
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (j < nj)
-                mma_mxf4_pair(tmem_base, sdesc_kmajor_sw128(a_s + j * 32), sdesc_kmajor_sw128(b_s + j * 32),
-                              idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 8, (kb | j) != 0 ? 1u : 0u);
-            }
-            const uint32_t eb = smem_u32(&empty_bar[stage]);
-            tc_commit_pair(mapa_shared(eb, 0));
-            tc_commit_pair(mapa_shared(eb, 1));
-          }
-          __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    // ───────── MMA issuer ─────────
+    const bool one = elect_one();
+    uint32_t acc_phase = 0;
+    constexpr uint32_t idesc[2] = {idesc_mxf4(MG_BM, S::BN, 0), idesc_mxf4(MG_BM, S::BN, 2)};
+    const uint64_t a0 = sdesc_kmajor_sw128(smem_u32(sA)), b0 = sdesc_kmajor_sw128(smem_u32(sB));
+    mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int, int kb, int s, uint32_t phase) {
+      if (kb == 0 && !mbar_wait(smem_u32(tempty_bar), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mbar_wait(smem_u32(&sff_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      tc_fence_after();
+      const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
+      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
+      if (one) {
+        mma_mxf4(0, a_d, b_d, idesc[0], tsfa, tsfb, kb != 0 ? 1u : 0u);
+        mma_mxf4(0, a_d + 2, b_d + 2, idesc[1], tsfa, tsfb, 1u);
+        if (2 * kb + 1 < (int)p.katoms) {                           // a whole stage
+          mma_mxf4(0, a_d + 4, b_d + 4, idesc[0], tsfa + 4, tsfb + 8, 1u);
+          mma_mxf4(0, a_d + 6, b_d + 6, idesc[1], tsfa + 4, tsfb + 8, 1u);
         }
-        if (lane == 0) {
-          tc_commit_pair(mapa_shared(smem_u32(tfull_bar), 0));
-          tc_commit_pair(mapa_shared(smem_u32(tfull_bar), 1));
-        }
-        __syncwarp();
-        acc_phase ^= 1;
+        tc_commit(smem_u32(&empty_bar[s]));
+        if (kb + 1 == n_kblk) tc_commit(smem_u32(tfull_bar));
       }
-    }
+      __syncwarp();
+      if (kb + 1 == n_kblk) acc_phase ^= 1;
+      return true;
+    });
   } else if (warp == COPIER) {
-    // ───────── scale copier (leader) ─────────
+    // ───────── scale copier ─────────
     // Slot s is rewritten only after full[s] of the next round, posted after empty[s], which the
     // MMA warp commits after the MMAs that read the slot.
-    if (leader) {
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int t = t0; t < total; t += step) {
-        for (int kb = 0; kb < n_kblk; ++kb) {
-          if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
-            const uint32_t sa = smem_u32(sSFA + stage * MG_SF_BYTES), sb = smem_u32(sSFB + stage * 2 * MG_SF_BYTES);
-#pragma unroll
-            for (int a = 0; a < 2; ++a) {
-              tc_cp_32x128b_warpx4_pair(tsfa + a * 4, sdesc_sf_chunk(sa + a * 512));
-              tc_cp_32x128b_warpx4_pair(tsfb + a * 8, sdesc_sf_chunk(sb + a * 512));
-              tc_cp_32x128b_warpx4_pair(tsfb + a * 8 + 4, sdesc_sf_chunk(sb + MG_SF_BYTES + a * 512));
-            }
-            tc_commit_pair(mapa_shared(smem_u32(&sff_bar[stage]), 0));
-          }
-          __syncwarp();
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    const bool one = elect_one();
+    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
+    mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int, int kb, int s, uint32_t phase) {
+      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      tc_fence_after();
+      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
+      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (2 * MG_SF_BYTES >> 4);
+      if (one) {
+        tc_cp_32x128b_warpx4(tsfa, sa);
+        tc_cp_32x128b_warpx4(tsfb, sb);
+        tc_cp_32x128b_warpx4(tsfb + 4, sb + (MG_SF_BYTES >> 4));
+        if (2 * kb + 1 < (int)p.katoms) {
+          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
+          tc_cp_32x128b_warpx4(tsfb + 8, sb + 32);
+          tc_cp_32x128b_warpx4(tsfb + 12, sb + (MG_SF_BYTES >> 4) + 32);
         }
+        tc_commit(smem_u32(&sff_bar[s]));
       }
-    }
+      __syncwarp();
+      return true;
+    });
   } else {
-    // ───────── epilogue (both CTAs, their own 128 tokens) ─────────
+    // ───────── epilogue ─────────
     const int q = warp & 3;                        // TMEM lane quarter of this warp
     const int slice = (warp - 2) >> 2;             // accumulator columns [64 * slice, +64)
-    const uint32_t tempty_leader = mapa_shared(smem_u32(tempty_bar), 0);
     uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
     uint32_t acc_phase = 0;
-    const int m0 = (int)crank * 128 + q * 32;
+    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
     for (int t = t0; t < total; t += step) {
-      const int tt = t / p.n_wt, wt = t % p.n_wt;
-      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const int wt = t % p.n_wt;
+      const MgTile tile = next;
+      if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
       if (!mbar_wait(smem_u32(tfull_bar), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
       acc_phase ^= 1;
       tc_fence_after();
       uint32_t r[64];
-      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(slice * 64);
+      const uint32_t taddr = ((uint32_t)(q * 32) << 16) + (uint32_t)(slice * 64);
       MHMOE_TMEM_LD_32x32b_X32(taddr, (r + 0));
       MHMOE_TMEM_LD_32x32b_X32(taddr + 32, (r + 32));
       tmem_wait_ld();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(tempty_leader);
-      if (m0 < tile.rows) mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * 256 + slice * 64, m0, lane, stg);
+      if (lane == 0) mbar_arrive(smem_u32(tempty_bar));
+      if (q * 32 < tile.rows)
+        mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * S::BN + slice * 64, q * 32, lane, stg);
     }
   }
-done:
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
-  if (leader && warp == 1 && lane == 0) {
-    tc_commit_pair(mapa_shared(smem_u32(&drain_bar[0]), 0));
+  if (warp == 1 && lane == 0) {
+    tc_commit(smem_u32(&drain_bar[0]));
     mbar_wait(smem_u32(&drain_bar[0]), 0, nullptr, 0, MHMOE_DRAIN_NS);
   }
-  if (leader && warp == COPIER && lane == 0) {
-    tc_commit_pair(mapa_shared(smem_u32(&drain_bar[1]), 0));
+  if (warp == COPIER && lane == 0) {
+    tc_commit(smem_u32(&drain_bar[1]));
     mbar_wait(smem_u32(&drain_bar[1]), 0, nullptr, 0, MHMOE_DRAIN_NS);
   }
   tc_fence_before();
-  cluster_sync();                                  // neither CTA leaves while the pair still uses it
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem_base, MG_TMEM_COLS);
+    tmem_dealloc(*tmem_slot, MG_TMEM_COLS);
   }
 }
 
@@ -474,7 +477,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   static_assert((3 * STAGES + 2 * NACC + 2) * 8 + 4 <= MG_MISC_BYTES, "barriers");
   static_assert(!SPLIT || BN * 128 * 4 <= STAGES * MG_A_BYTES, "partial sums lie over operand A's stages");
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -499,7 +502,6 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
 
   const int n_tiles = p.n_tiles ? min(*p.n_tiles, p.max_tiles) : p.max_tiles;
   const int total = n_tiles * p.n_wt;
@@ -517,95 +519,90 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
 
   if (warp == 0) {
     // ───────── producer ─────────
-    int stage = 0;
-    uint32_t phase = 0;
+    const bool one = elect_one();
     int64_t issued = 0;
-    bool ok = true;
     const uint32_t wblk = (uint32_t)((p.N + 127) / 128);
-    for (int64_t t = t0; ok && t < total; t += step) {
-      const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
-      const MgTile tile = mg_tile<S::SLOT>(p, tt);
-      const int wrow = tile.e * p.N + wt * 128;
-      const uint8_t* sf_t = p.sf_tok + (uint64_t)tile.slot * p.katoms * 512;
-      const uint8_t* sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wt) * p.katoms * 512;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&empty_bar[stage]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) {
-          const uint32_t fb = smem_u32(&full_bar[stage]);
-          const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;  // atoms of this stage
-          mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * 2);
-          tma_load_2d(smem_u32(sA + stage * MG_A_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
-          tma_load_2d(smem_u32(sB + stage * S::B_BYTES), &tmT, fb, kb * (MG_BK / 2), (int)tile.row0);
-          bulk_load(smem_u32(sSFA + stage * MG_SF_BYTES), sf_w + kb * 1024, sfn, fb);
-          bulk_load(smem_u32(sSFB + stage * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
-        }
-        __syncwarp();
-        ++issued;
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int trow = 0, wrow = 0;
+    const uint8_t *sf_t = nullptr, *sf_w = nullptr;
+    mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int t, int kb, int s, uint32_t phase) {
+      if (kb == kb0) {
+        const int wt = t % p.n_wt;
+        trow = (int)next.row0;
+        wrow = next.e * p.N + wt * 128;
+        sf_t = p.sf_tok + (uint64_t)next.slot * p.katoms * 512;
+        sf_w = p.sf_w + ((uint64_t)next.e * wblk + wt) * p.katoms * 512;
+        if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
       }
-    }
+      if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (one) {
+        const uint32_t fb = smem_u32(&full_bar[s]);
+        const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;      // atoms of this stage
+        mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * 2);
+        tma_load_2d(smem_u32(sA + s * MG_A_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
+        tma_load_2d(smem_u32(sB + s * S::B_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
+        bulk_load(smem_u32(sSFA + s * MG_SF_BYTES), sf_w + kb * 1024, sfn, fb);
+        bulk_load(smem_u32(sSFB + s * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
+      }
+      __syncwarp();
+      ++issued;
+      return true;
+    });
     // every copy lands before the CTA can exit (returns at once unless a consumer gave up)
     for (int64_t i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i)
       mbar_wait(smem_u32(&full_bar[i % STAGES]), (uint32_t)((i / STAGES) & 1), nullptr, 0, MHMOE_DRAIN_NS);
   } else if (warp == 1) {
     // ───────── MMA issuer ─────────
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
+    const bool one = elect_one();
+    uint32_t acc = 0, acc_phase = 0;
     constexpr uint32_t idesc[2] = {idesc_mxf4(MG_BM, BN, 0), idesc_mxf4(MG_BM, BN, 2)};
-    for (int64_t t = t0; t < total; t += step) {
-      if (!mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
+    const uint64_t a0 = sdesc_kmajor_sw128(smem_u32(sA)), b0 = sdesc_kmajor_sw128(smem_u32(sB));
+    mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
+      if (kb == kb0 && !mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout))
+        return false;
+      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mbar_wait(smem_u32(&sff_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       tc_fence_after();
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-        if (!mbar_wait(smem_u32(&sff_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
-          const uint32_t a_s = smem_u32(sA + stage * MG_A_BYTES);
-          const uint32_t b_s = smem_u32(sB + stage * S::B_BYTES);
-          const int nj = (int)min(4u, 2 * (p.katoms - 2 * kb));    // 64-column steps of this stage
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (j < nj)
-              mma_mxf4(tmem_base + acc * BN, sdesc_kmajor_sw128(a_s + j * 32), sdesc_kmajor_sw128(b_s + j * 32),
-                       idesc[j & 1], tsfa + (j >> 1) * 4, tsfb + (j >> 1) * 4, (kb > kb0 || j > 0) ? 1u : 0u);
-          }
-          tc_commit(smem_u32(&empty_bar[stage]));
+      const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
+      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8, d = acc * BN;
+      if (one) {
+        mma_mxf4(d, a_d, b_d, idesc[0], tsfa, tsfb, kb != kb0 ? 1u : 0u);
+        mma_mxf4(d, a_d + 2, b_d + 2, idesc[1], tsfa, tsfb, 1u);
+        if (2 * kb + 1 < (int)p.katoms) {                           // a whole stage
+          mma_mxf4(d, a_d + 4, b_d + 4, idesc[0], tsfa + 4, tsfb + 4, 1u);
+          mma_mxf4(d, a_d + 6, b_d + 6, idesc[1], tsfa + 4, tsfb + 4, 1u);
         }
-        __syncwarp();
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        tc_commit(smem_u32(&empty_bar[s]));
+        if (kb + 1 == kb1) tc_commit(smem_u32(&tfull_bar[acc]));
       }
-      if (lane == 0) tc_commit(smem_u32(&tfull_bar[acc]));
       __syncwarp();
-      if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
-    }
+      if (kb + 1 == kb1 && ++acc == NACC) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+      return true;
+    });
   } else if (warp == COPIER) {
     // ───────── scale copier ─────────
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int64_t t = t0; t < total; t += step) {
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(smem_u32(&full_bar[stage]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) goto done;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t tsfa = tmem_base + S::SF_COL0 + stage * S::SF_COLS, tsfb = tsfa + 8;
-          const uint32_t sa = smem_u32(sSFA + stage * MG_SF_BYTES), sb = smem_u32(sSFB + stage * MG_SF_BYTES);
-#pragma unroll
-          for (int a = 0; a < 2; ++a) {
-            if (2 * kb + a < (int)p.katoms) {
-              tc_cp_32x128b_warpx4(tsfa + a * 4, sdesc_sf_chunk(sa + a * 512));
-              tc_cp_32x128b_warpx4(tsfb + a * 4, sdesc_sf_chunk(sb + a * 512));
-            }
-          }
-          tc_commit(smem_u32(&sff_bar[stage]));
+    const bool one = elect_one();
+    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
+    mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
+      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      tc_fence_after();
+      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
+      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (MG_SF_BYTES >> 4);
+      if (one) {
+        tc_cp_32x128b_warpx4(tsfa, sa);
+        tc_cp_32x128b_warpx4(tsfb, sb);
+        if (2 * kb + 1 < (int)p.katoms) {
+          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
+          tc_cp_32x128b_warpx4(tsfb + 4, sb + 32);
         }
-        __syncwarp();
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        tc_commit(smem_u32(&sff_bar[s]));
       }
-    }
+      __syncwarp();
+      return true;
+    });
   } else {
     // ───────── epilogue ─────────
     const int q = warp & 3;                    // TMEM lane quarter of this warp
@@ -614,14 +611,16 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int64_t t = t0; t < total; t += step) {
-      const int tt = (int)(t / p.n_wt), wt = (int)(t % p.n_wt);
-      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    for (int t = t0; t < total; t += step) {
+      const int wt = t % p.n_wt;
+      const MgTile tile = next;
+      if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
       const int n0 = wt * 128 + q * 32;
       const float b = p.bias && n0 + lane < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n0 + lane) : 0.f;
       if (!mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
       tc_fence_after();
-      const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
+      const uint32_t taddr = ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
       for (int j0 = part * NC; j0 < BN && j0 < tile.rows; j0 += NC * (EPW / 4)) {
         uint32_t r[NC];
         if constexpr (NC == 16) MHMOE_TMEM_LD_32x32b_X16(taddr + j0, r);
@@ -642,7 +641,6 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
     }
   }
-done:
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
   if (warp == 1 && lane == 0) {
     tc_commit(smem_u32(&drain_bar[0]));
@@ -656,7 +654,7 @@ done:
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, MG_TMEM_COLS);
+    tmem_dealloc(*tmem_slot, MG_TMEM_COLS);
   }
   if constexpr (SPLIT) {
     cluster_sync();
@@ -808,8 +806,7 @@ __global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>
   if (!ok && lane == 0) record_error(p.status, MHMOE_ERR_ARGS);
   const typename MxType<DT>::T* xr = x + (ok ? src : 0) * p.x_stride;
   uint8_t* d = p.data + r * (int64_t)p.katoms * 64;
-  const int blocks = (p.slot_rows + 127) / 128;
-  uint8_t* s = p.sf + ((uint64_t)slot * blocks + (m >> 7)) * p.katoms * 512 + (m & 31) * 16 + ((m >> 5) & 3) * 4;
+  uint8_t* s = p.sf + (uint64_t)slot * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
 #pragma unroll 2
   for (uint32_t c0 = lane * 16; c0 < (p.katoms + 3) / 4 * 512; c0 += 512) {
     MxRaw16<typename MxType<DT>::T> v;
@@ -847,10 +844,10 @@ MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
     g.flat = true;
     g.bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   } else {
-    g.flat = tiles_of(256) * ceil_div(N, 256) < sms / 2;
+    g.flat = tiles_of(128) * ceil_div(N, 256) < sms;
     g.bn = 128;
   }
-  g.slot_rows = g.flat ? g.bn : 256;
+  g.slot_rows = g.bn;
   g.tiles = tiles_of(g.slot_rows);
   g.slots = grouped ? R / g.slot_rows + n + 1 : g.tiles;
   g.n_wt = (int)ceil_div(N, g.flat ? 128 : 256);
@@ -868,37 +865,23 @@ MgScratch mg_scratch(const MgPlan& g, int64_t R, int64_t katoms, bool grouped) {
   MgScratch s;
   s.data = 0;
   s.sf = up((size_t)R * katoms * 64);
-  const int64_t blocks = grouped ? g.slots * ceil_div(g.slot_rows, 128) : ceil_div(R, 128);
-  s.tiles = s.sf + up((size_t)blocks * katoms * 512);
+  s.tiles = s.sf + up((size_t)(grouped ? g.slots : ceil_div(R, 128)) * katoms * 512);
   s.count = s.tiles + (grouped ? up((size_t)g.tiles * sizeof(int4)) : 0);
   s.bytes = s.count + (grouped ? 256 : 0);
   return s;
 }
 
 template <bool OUT32, bool SWIGLU>
-cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const CUtensorMap& tsft, const CUtensorMap& tsfw,
-                        const MgParams& p, const MgPlan& g, cudaStream_t st) {
+cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                        cudaStream_t st) {
   using S = WideShape;
   auto kernel = mx_wide_kernel<OUT32, SWIGLU>;
-  // per device: the shared-memory attribute and the clusters that fit at once
   static PerDeviceOnce once;
-  static int max_clusters[MHMOE_MAX_DEVICES] = {};
-  const cudaError_t attr = once.run([&](int dev) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * (num_sms() / 2));
-    cfg.blockDim = dim3(S::THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    e = cudaOccupancyMaxActiveClusters(&max_clusters[dev], kernel, &cfg);
-    if (e == cudaSuccess && max_clusters[dev] <= 0) e = cudaErrorInvalidConfiguration;
-    return e;
-  });
+  const cudaError_t attr = once.run(
+      [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
   if (attr != cudaSuccess) return attr;
-  int dev = 0;
-  cudaGetDevice(&dev);
-  const int64_t clusters = std::min<int64_t>(max_clusters[dev], g.tiles * g.n_wt);
-  return launch_pdl(kernel, dim3((unsigned)(2 * clusters)), dim3(S::THREADS), S::SMEM, st, tt, tw, tsft, tsfw, p);
+  return launch_pdl(kernel, dim3((unsigned)std::min<int64_t>(num_sms(), g.tiles * g.n_wt)), dim3(S::THREADS), S::SMEM, st,
+                    tt, tw, p);
 }
 
 template <int BN, bool SPLIT, bool OUT32>
@@ -1017,30 +1000,18 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
   a.status = p.status;
   a.timeout_ns = p.timeout_ns;
   CUtensorMap tt, tw;
-  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)std::min(g.slot_rows, 128)) !=
-          cudaSuccess ||
-      encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, 128) != cudaSuccess)
+  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)g.slot_rows) != cudaSuccess ||
+      encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, g.flat ? 128 : 256) != cudaSuccess)
     return MHMOE_ERR_DRIVER;
-  if (g.flat) {
+  if (g.flat)
     *cerr = g.bn == 16   ? launch_flat<16>(tt, tw, a, g, st)
             : g.bn == 32 ? launch_flat<32>(tt, tw, a, g, st)
             : g.bn == 64 ? launch_flat<64>(tt, tw, a, g, st)
                          : launch_flat<128>(tt, tw, a, g, st);
-  } else {
-    const int64_t blocks = grouped ? g.slots * 2 : ceil_div(p.R, 128), wblk = ceil_div(p.N, 128);
-    CUtensorMap tsft, tsfw;
-    if (encode_tmap_2d(&tsft, a.sf_tok, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 256, (uint64_t)blocks * katoms * 2, 256, 256, 4,
-                       false) != cudaSuccess ||
-        encode_tmap_2d(&tsfw, p.w_sf, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, 256, (uint64_t)p.n * wblk * katoms * 2, 256, 256,
-                       4, false) != cudaSuccess)
-      return MHMOE_ERR_DRIVER;
-    if (p.y_dtype == DT_F32)
-      *cerr = p.act ? launch_wide<true, true>(tt, tw, tsft, tsfw, a, g, st)
-                    : launch_wide<true, false>(tt, tw, tsft, tsfw, a, g, st);
-    else
-      *cerr = p.act ? launch_wide<false, true>(tt, tw, tsft, tsfw, a, g, st)
-                    : launch_wide<false, false>(tt, tw, tsft, tsfw, a, g, st);
-  }
+  else if (p.y_dtype == DT_F32)
+    *cerr = p.act ? launch_wide<true, true>(tt, tw, a, g, st) : launch_wide<true, false>(tt, tw, a, g, st);
+  else
+    *cerr = p.act ? launch_wide<false, true>(tt, tw, a, g, st) : launch_wide<false, false>(tt, tw, a, g, st);
   return *cerr == cudaSuccess ? MHMOE_OK : MHMOE_ERR_LAUNCH;
 }
 
