@@ -25,7 +25,7 @@ constexpr int MG_BM = 128;                  // rows of operand A a CTA
 constexpr int MG_BK = 256;                  // columns of a stage: 128 B a row
 constexpr int MG_A_BYTES = MG_BM * MG_BK / 2;
 constexpr int MG_SF_BYTES = 2 * 512;        // scales of 128 rows x 256 columns: two atoms
-constexpr int MG_STG_BYTES = 1024;          // store staging per epilogue warp: 32 rows x 32 B
+constexpr int MG_STG_WIDE = 32, MG_STG_FLAT = 64;   // bytes of a row of an epilogue warp's store staging, 32 rows
 constexpr int MG_MISC_BYTES = 512;          // barriers, TMEM slot
 constexpr int MG_TMEM_COLS = 512;
 
@@ -36,7 +36,7 @@ struct WideShape {
   static constexpr int STAGES = 4;
   static constexpr int EPW = 16;                                // epilogue warps: 64 columns each
   static constexpr int THREADS = 32 * (3 + EPW);
-  static constexpr int SMEM = STAGES * STAGE + EPW * MG_STG_BYTES + MG_MISC_BYTES + 1024;
+  static constexpr int SMEM = STAGES * STAGE + EPW * 32 * MG_STG_WIDE + MG_MISC_BYTES + 1024;
   static constexpr int SF_COLS = 24, SF_COL0 = 256;             // TMEM: accumulator, then the stages' scales
   static_assert(SMEM <= 227 * 1024, "shared memory");
   static_assert(SF_COL0 + STAGES * SF_COLS <= MG_TMEM_COLS, "TMEM");
@@ -50,7 +50,7 @@ struct FlatShape {
   static constexpr int EPW = BN >= 64 ? 8 : 4;
   static constexpr int STAGES = BN <= 16 ? 9 : BN <= 32 ? 8 : BN <= 64 ? 7 : 5;
   static constexpr int THREADS = 32 * (3 + EPW);
-  static constexpr int SMEM = STAGES * STAGE + EPW * MG_STG_BYTES + MG_MISC_BYTES + 1024;
+  static constexpr int SMEM = STAGES * STAGE + EPW * 32 * MG_STG_FLAT + MG_MISC_BYTES + 1024;
   static constexpr int NACC = 2;                                // accumulators in TMEM
   static constexpr int SF_COLS = 16, SF_COL0 = NACC * BN;
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -100,13 +100,15 @@ __device__ __forceinline__ MgTile mg_tile(const MgParams& p, int tt) {
   return t;
 }
 
-__device__ __forceinline__ uint32_t mg_pack16(float a, float b, bool half) {
-  if (half) {
+template <int OUT>
+__device__ __forceinline__ uint32_t mg_pack16(float a, float b) {
+  if constexpr (OUT == DT_F16) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 __device__ __forceinline__ void mg_store(void* y, int dtype, int64_t at, float v) {
@@ -115,29 +117,36 @@ __device__ __forceinline__ void mg_store(void* y, int dtype, int64_t at, float v
   else static_cast<__half*>(y)[at] = __float2half_rn(v);
 }
 
-// Byte offset of 16-B chunk k (0, 1) of a staging row of 32 B: four rows fill the 32 banks once.
-__device__ __forceinline__ int mg_stg(int row, int k) { return row * 32 + ((k ^ ((row >> 2) & 1)) << 4); }
+// Byte offset of 16-B chunk k of a staging row of ROWB bytes, so that eight threads' chunks (the same
+// k of eight rows, or all of neighbouring rows) lie in different banks.
+template <int ROWB>
+__device__ __forceinline__ int mg_stg(int row, int k) {
+  return row * ROWB + ((k ^ (ROWB == 32 ? (row >> 2) & 1 : (row >> 1) & 3)) << 4);
+}
 
-// 32 rows x 32 B of the warp's staging to the rows row0 + 0.. of y, `rows` of them, from output
+// 32 rows x ROWB bytes of the warp's staging to the rows row0 + 0.. of y, `rows` of them, from output
 // column c0; `width` outputs a row are valid.
-template <int ESZ>
+template <int ESZ, int ROWB>
 __device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* stg, int64_t row0, int rows, int c0,
                                               int width, int lane) {
   uint8_t* y = static_cast<uint8_t*>(p.y);
+  constexpr int K = ROWB / 16, P16 = 16 / ESZ;
   if (p.y_vec) {
+    const int k = lane % K;
+    uint8_t* dst = y + ((row0 + lane / K) * p.y_stride + c0 + k * P16) * ESZ;
+    const int64_t hop = (int64_t)(32 / K) * p.y_stride * ESZ;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = i * 16 + (lane >> 1), k = lane & 1;
-      if (row < rows && k * (16 / ESZ) < width)
-        *reinterpret_cast<uint4*>(y + ((row0 + row) * p.y_stride + c0 + k * (16 / ESZ)) * ESZ) =
-            *reinterpret_cast<const uint4*>(stg + mg_stg(row, k));
+    for (int i = 0; i < K; ++i, dst += hop) {
+      const int row = i * (32 / K) + lane / K;
+      if (row < rows && k * P16 < width)
+        *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(stg + mg_stg<ROWB>(row, k));
     }
   } else {
-    constexpr int PER = 32 / ESZ;                   // one output a lane
+    constexpr int PER = ROWB / ESZ;                 // one output a lane
     const int col = lane % PER;
     for (int row = lane / PER; row < rows; row += 32 / PER) {
       if (col >= width) break;
-      const uint8_t* src = stg + mg_stg(row, col * ESZ >> 4) + (col * ESZ & 15);
+      const uint8_t* src = stg + mg_stg<ROWB>(row, col * ESZ >> 4) + (col * ESZ & 15);
       uint8_t* dst = y + ((row0 + row) * p.y_stride + c0 + col) * ESZ;
       if constexpr (ESZ == 4) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(src);
       else *reinterpret_cast<uint16_t*>(dst) = *reinterpret_cast<const uint16_t*>(src);
@@ -146,10 +155,11 @@ __device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* 
 }
 
 // Wide epilogue: 32 token rows (one a thread) x 64 accumulator columns from weight row col0.
-template <bool OUT32, bool SWIGLU>
+template <int OUT, bool SWIGLU>
 __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, uint32_t (&r)[64], int col0,
                                                  int m0, int lane, uint8_t* stg) {
-  constexpr int PER = OUT32 ? 8 : 16;               // outputs of a 32-B chunk
+  constexpr int ESZ = OUT == DT_F32 ? 4 : 2;
+  constexpr int PER = MG_STG_WIDE / ESZ;            // outputs of a staging row
   constexpr int ACC = SWIGLU ? 2 * PER : PER;       // accumulator columns behind them
   const int n_out = SWIGLU ? p.N / 2 : p.N;
   if (p.bias) {
@@ -158,7 +168,6 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
     for (int i = 0; i < 64; ++i)
       if (col0 + i < p.N) r[i] = __float_as_uint(__uint_as_float(r[i]) + __ldg(bias + i));
   }
-  const bool half = p.y_dtype == DT_F16;
   float rw = 1.f;
   if (p.row_weights && m0 + lane < t.rows) rw = __ldg(p.row_weights + t.row0 + m0 + lane);
 #pragma unroll
@@ -177,29 +186,28 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
     }
     __syncwarp();                                   // the chunk before has left the staging
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < MG_STG_WIDE / 16; ++k) {
       uint32_t w[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (OUT32) w[j] = __float_as_uint(v[4 * k + j]);
-        else w[j] = mg_pack16(v[8 * k + 2 * j], v[8 * k + 2 * j + 1], half);
+        if constexpr (OUT == DT_F32) w[j] = __float_as_uint(v[4 * k + j]);
+        else w[j] = mg_pack16<OUT>(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
       }
-      *reinterpret_cast<uint4*>(stg + mg_stg(lane, k)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(stg + mg_stg<MG_STG_WIDE>(lane, k)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
     __syncwarp();
     const int o0 = SWIGLU ? (col0 + c * ACC) / 2 : col0 + c * ACC;
-    mg_store_rows<OUT32 ? 4 : 2>(p, stg, t.row0 + m0, min(32, t.rows - m0), o0, n_out - o0, lane);
+    mg_store_rows<ESZ, MG_STG_WIDE>(p, stg, t.row0 + m0, min(32, t.rows - m0), o0, n_out - o0, lane);
   }
 }
 
 // Flat epilogue: one weight row n a thread (32 of the warp's from n0) x NC token columns from j0.
-// The transposed outputs go through the staging in passes of 32 B a token row.
-template <int NC, bool OUT32>
+// The transposed outputs go through the staging in passes of 64 B a token row.
+template <int NC, int OUT>
 __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile& t, const uint32_t (&r)[NC], int j0,
                                                  int n0, float b, int lane, uint8_t* stg) {
-  using U = typename std::conditional<OUT32, float, uint16_t>::type;
-  constexpr int ESZ = OUT32 ? 4 : 2, PER = 32 / ESZ;
-  const bool half = p.y_dtype == DT_F16;
+  using U = typename std::conditional<OUT == DT_F32, float, uint16_t>::type;
+  constexpr int ESZ = OUT == DT_F32 ? 4 : 2, PER = MG_STG_FLAT / ESZ;
   const int rows = min(NC, t.rows - j0);
   // a row's weight, from the lane that holds it
   float rw = 1.f;
@@ -214,20 +222,21 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
   const int n_out = p.act ? p.N / 2 : p.N, o0 = p.act ? n0 / 2 : n0;
   const int width = p.act ? 16 : 32;                // outputs of the warp a token row
 #pragma unroll
-  for (int c = 0; c < 32 / PER; ++c) {
+  for (int c = 0; c < 32 / PER; ++c) {              // fp32 without activation: two passes of 16 outputs
     if (c * PER >= width) break;
     const int at = (p.act ? lane >> 1 : lane) - c * PER;
     __syncwarp();
     if (at >= 0 && at < PER && !(p.act && (lane & 1))) {
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
-        U* dst = reinterpret_cast<U*>(stg + mg_stg(j, at * ESZ >> 4) + (at * ESZ & 15));
-        if constexpr (OUT32) *dst = v[j];
-        else *dst = (uint16_t)mg_pack16(v[j], 0.f, half);
+        U* dst = reinterpret_cast<U*>(stg + mg_stg<MG_STG_FLAT>(j, at * ESZ >> 4) + (at * ESZ & 15));
+        if constexpr (OUT == DT_F32) *dst = v[j];
+        else *dst = (uint16_t)mg_pack16<OUT>(v[j], 0.f);
       }
     }
     __syncwarp();
-    mg_store_rows<ESZ>(p, stg, t.row0 + j0, rows, o0 + c * PER, min(width - c * PER, n_out - o0 - c * PER), lane);
+    mg_store_rows<ESZ, MG_STG_FLAT>(p, stg, t.row0 + j0, rows, o0 + c * PER, min(width - c * PER, n_out - o0 - c * PER),
+                                    lane);
   }
 }
 
@@ -262,7 +271,12 @@ __device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int k
 
 // Wide kernel.  tmT: token rows [R, cols_p/2], box 128 B x 128; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 256.
-template <bool OUT32, bool SWIGLU>
+//
+// One accumulator: its 256 columns leave for registers in 430 clocks, after which the next tile's MMAs
+// run under the epilogue.  (Two that share 48 columns, the scales in two slots, hid most of the
+// 430, but the barriers they need made both the MMA warp and the epilogue slower: 187 against 165 us
+// for 131072 expert rows x 2048 x 1024, 112 against 109 for 8192^2 x 4096.)
+template <int OUT, bool SWIGLU>
 __global__ void __launch_bounds__(WideShape::THREADS, 1)
     mx_wide_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ MgParams p) {
@@ -277,7 +291,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
   uint8_t* sSFA = sB + STAGES * S::B_BYTES;
   uint8_t* sSFB = sSFA + STAGES * MG_SF_BYTES;
   uint8_t* sSTG = sSFB + STAGES * 2 * MG_SF_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * 32 * MG_STG_WIDE);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sff_bar = empty_bar + STAGES;          // the stage's scales are in TMEM
   uint64_t* tfull_bar = sff_bar + STAGES;
@@ -410,7 +424,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     // ───────── epilogue ─────────
     const int q = warp & 3;                        // TMEM lane quarter of this warp
     const int slice = (warp - 2) >> 2;             // accumulator columns [64 * slice, +64)
-    uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
+    uint8_t* stg = sSTG + (warp - 2) * 32 * MG_STG_WIDE;
     uint32_t acc_phase = 0;
     MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
     for (int t = t0; t < total; t += step) {
@@ -429,9 +443,10 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(tempty_bar));
       if (q * 32 < tile.rows)
-        mg_wide_epilogue<OUT32, SWIGLU>(p, tile, r, wt * S::BN + slice * 64, q * 32, lane, stg);
+        mg_wide_epilogue<OUT, SWIGLU>(p, tile, r, wt * S::BN + slice * 64, q * 32, lane, stg);
     }
   }
+
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
   if (warp == 1 && lane == 0) {
     tc_commit(smem_u32(&drain_bar[0]));
@@ -452,7 +467,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
 // Flat kernel.  tmT: token rows [R, cols_p/2], box 128 B x BN; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 128.  SPLIT: a cluster of CTAs shares one work item along the columns; their partial
 // accumulators meet in distributed shared memory and are summed in the order of the ranks.
-template <int BN, bool SPLIT, bool OUT32>
+template <int BN, bool SPLIT, int OUT>
 __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     mx_flat_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ MgParams p) {
@@ -467,7 +482,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   uint8_t* sSFA = sB + STAGES * S::B_BYTES;
   uint8_t* sSFB = sSFA + STAGES * MG_SF_BYTES;
   uint8_t* sSTG = sSFB + STAGES * MG_SF_BYTES;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * MG_STG_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * 32 * MG_STG_FLAT);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* sff_bar = empty_bar + STAGES;      // the stage's scales are in TMEM
   uint64_t* tfull_bar = sff_bar + STAGES;      // [NACC]
@@ -608,7 +623,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     const int q = warp & 3;                    // TMEM lane quarter of this warp
     const int part = (warp - 2) >> 2;          // with 8 warps: every other chunk of columns
     constexpr int NC = BN < 32 ? BN : 32;
-    uint8_t* stg = sSTG + (warp - 2) * MG_STG_BYTES;
+    uint8_t* stg = sSTG + (warp - 2) * 32 * MG_STG_FLAT;
     int acc = 0;
     uint32_t acc_phase = 0;
     MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
@@ -632,7 +647,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
 #pragma unroll
           for (int j = 0; j < NC; ++j) red[(j0 + j) * 128 + q * 32 + lane] = __uint_as_float(r[j]);
         } else {
-          if (n0 < p.N) mg_flat_epilogue<NC, OUT32>(p, tile, r, j0, n0, b, lane, stg);
+          if (n0 < p.N) mg_flat_epilogue<NC, OUT>(p, tile, r, j0, n0, b, lane, stg);
         }
       }
       tc_fence_before();
@@ -641,6 +656,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       if (++acc == NACC) { acc = 0; acc_phase ^= 1; }
     }
   }
+
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
   if (warp == 1 && lane == 0) {
     tc_commit(smem_u32(&drain_bar[0]));
@@ -838,12 +854,16 @@ MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
   MgPlan g;
   const int64_t avg = grouped ? ceil_div(R, n) : R;
   auto tiles_of = [&](int64_t slot) { return grouped ? R / slot + std::min<int64_t>(n, R) : ceil_div(R, slot); };
-  if (avg <= 64 || (!grouped && R <= 128)) {
+  if (grouped ? avg <= 16 : R <= 128) {
     // a few rows per matrix: one flat tile holds them
     const int64_t want = grouped ? avg + avg / 2 : avg;
     g.flat = true;
     g.bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   } else {
+    // Above that the wide tile, however few of its 128 rows an expert fills: its 256 weight rows
+    // stream past in 700 clocks a stage, faster than HBM delivers them (128 experts of 2048 x 1024,
+    // 4096 rows: 34 us wide, 45 and 57 flat with 128 and 64 columns).  Flat where the wide tiles
+    // would not reach every SM.
     g.flat = tiles_of(128) * ceil_div(N, 256) < sms;
     g.bn = 128;
   }
@@ -871,11 +891,11 @@ MgScratch mg_scratch(const MgPlan& g, int64_t R, int64_t katoms, bool grouped) {
   return s;
 }
 
-template <bool OUT32, bool SWIGLU>
+template <int OUT, bool SWIGLU>
 cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
                         cudaStream_t st) {
   using S = WideShape;
-  auto kernel = mx_wide_kernel<OUT32, SWIGLU>;
+  auto kernel = mx_wide_kernel<OUT, SWIGLU>;
   static PerDeviceOnce once;
   const cudaError_t attr = once.run(
       [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
@@ -884,11 +904,11 @@ cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
                     tt, tw, p);
 }
 
-template <int BN, bool SPLIT, bool OUT32>
+template <int BN, bool SPLIT, int OUT>
 cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
                         cudaStream_t st) {
   using S = FlatShape<BN>;
-  auto kernel = mx_flat_kernel<BN, SPLIT, OUT32>;
+  auto kernel = mx_flat_kernel<BN, SPLIT, OUT>;
   static PerDeviceOnce once;
   const cudaError_t attr = once.run(
       [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
@@ -919,9 +939,16 @@ cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
 template <int BN>
 cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
                         cudaStream_t st) {
-  if (g.split > 1) return launch_flat<BN, true, false>(tt, tw, p, g, st);
-  return p.y_dtype == DT_F32 ? launch_flat<BN, false, true>(tt, tw, p, g, st)
-                             : launch_flat<BN, false, false>(tt, tw, p, g, st);
+  if (g.split > 1) return launch_flat<BN, true, DT_F32>(tt, tw, p, g, st);      // stores by p.y_dtype
+  return p.y_dtype == DT_F32    ? launch_flat<BN, false, DT_F32>(tt, tw, p, g, st)
+         : p.y_dtype == DT_BF16 ? launch_flat<BN, false, DT_BF16>(tt, tw, p, g, st)
+                                : launch_flat<BN, false, DT_F16>(tt, tw, p, g, st);
+}
+
+template <int OUT>
+cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
+                        cudaStream_t st) {
+  return p.act ? launch_wide<OUT, true>(tt, tw, p, g, st) : launch_wide<OUT, false>(tt, tw, p, g, st);
 }
 
 }  // namespace
@@ -1008,10 +1035,10 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
             : g.bn == 32 ? launch_flat<32>(tt, tw, a, g, st)
             : g.bn == 64 ? launch_flat<64>(tt, tw, a, g, st)
                          : launch_flat<128>(tt, tw, a, g, st);
-  else if (p.y_dtype == DT_F32)
-    *cerr = p.act ? launch_wide<true, true>(tt, tw, a, g, st) : launch_wide<true, false>(tt, tw, a, g, st);
   else
-    *cerr = p.act ? launch_wide<false, true>(tt, tw, a, g, st) : launch_wide<false, false>(tt, tw, a, g, st);
+    *cerr = p.y_dtype == DT_F32    ? launch_wide<DT_F32>(tt, tw, a, g, st)
+            : p.y_dtype == DT_BF16 ? launch_wide<DT_BF16>(tt, tw, a, g, st)
+                                   : launch_wide<DT_F16>(tt, tw, a, g, st);
   return *cerr == cudaSuccess ? MHMOE_OK : MHMOE_ERR_LAUNCH;
 }
 
