@@ -13,8 +13,9 @@
 //   flat   128 weight rows x 16..128 tokens: with a few tokens the instruction's 128 lanes are
 //          filled by the weights, which is what a decode step streams.  A cluster may share an
 //          item along the columns.
-// Warp roles: 0 TMA producer, 1 TMEM owner and MMA issuer, then the epilogue warps, last the
-// copier of scale atoms into TMEM (their own warp, so that copies run beside the MMAs).
+// Warp roles: 0 TMA producer, 1 TMEM owner and issuer of the scale copies into TMEM and the MMAs (the
+// tensor pipe keeps their order; a warp of its own for the copies, as the NVFP4 kernel has for its
+// twice as many, measured 2 % slower here), then the epilogue warps.
 #include "mxfp4.cuh"
 
 namespace mhmoe {
@@ -35,7 +36,7 @@ struct WideShape {
   static constexpr int STAGE = MG_A_BYTES + B_BYTES + 3 * MG_SF_BYTES;
   static constexpr int STAGES = 4;
   static constexpr int EPW = 16;                                // epilogue warps: 64 columns each
-  static constexpr int THREADS = 32 * (3 + EPW);
+  static constexpr int THREADS = 32 * (2 + EPW);
   static constexpr int SMEM = STAGES * STAGE + EPW * 32 * MG_STG_WIDE + MG_MISC_BYTES + 1024;
   static constexpr int SF_COLS = 24, SF_COL0 = 256;             // TMEM: accumulator, then the stages' scales
   static_assert(SMEM <= 227 * 1024, "shared memory");
@@ -49,7 +50,7 @@ struct FlatShape {
   static constexpr int STAGE = MG_A_BYTES + B_BYTES + 2 * MG_SF_BYTES;
   static constexpr int EPW = BN >= 64 ? 8 : 4;
   static constexpr int STAGES = BN <= 16 ? 9 : BN <= 32 ? 8 : BN <= 64 ? 7 : 5;
-  static constexpr int THREADS = 32 * (3 + EPW);
+  static constexpr int THREADS = 32 * (2 + EPW);
   static constexpr int SMEM = STAGES * STAGE + EPW * 32 * MG_STG_FLAT + MG_MISC_BYTES + 1024;
   static constexpr int NACC = 2;                                // accumulators in TMEM
   static constexpr int SF_COLS = 16, SF_COL0 = NACC * BN;
@@ -240,7 +241,7 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
   }
 }
 
-// The producer, copier and MMA warps share their schedulers with busy epilogue warps, so every
+// The producer and MMA warps share their schedulers with busy epilogue warps, so every
 // instruction of theirs between two asynchronous operations costs tensor time (a loop over the
 // stages with descriptors made on the way ran 803 clocks a stage of 8192^2 x 4096, this form 700).
 // Hence: the stages are unrolled, so that barriers, descriptors and TMEM columns are constants
@@ -272,7 +273,7 @@ __device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int k
 // Wide kernel.  tmT: token rows [R, cols_p/2], box 128 B x 128; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 256.
 //
-// One accumulator: its 256 columns leave for registers in 430 clocks, after which the next tile's MMAs
+// One accumulator: its 256 columns leave for registers in about 400 clocks, after which the next tile's MMAs
 // run under the epilogue.  (Two that share 48 columns, the scales in two slots, hid most of the
 // 430, but the barriers they need made both the MMA warp and the epilogue slower: 187 against 165 us
 // for 131072 expert rows x 2048 x 1024, 112 against 109 for 8192^2 x 4096.)
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
   pdl_wait();
   pdl_trigger();
   using S = WideShape;
-  constexpr int STAGES = S::STAGES, EPW = S::EPW, COPIER = 2 + EPW;
+  constexpr int STAGES = S::STAGES, EPW = S::EPW;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -293,12 +294,11 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
   uint8_t* sSTG = sSFB + STAGES * 2 * MG_SF_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * 32 * MG_STG_WIDE);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* sff_bar = empty_bar + STAGES;          // the stage's scales are in TMEM
-  uint64_t* tfull_bar = sff_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 1;
-  uint64_t* drain_bar = tempty_bar + 1;            // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
-  static_assert((3 * STAGES + 4) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  uint64_t* drain_bar = tempty_bar + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  static_assert((2 * STAGES + 3) * 8 + 4 <= MG_MISC_BYTES, "barriers");
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
   const int lane = threadIdx.x & 31;
@@ -306,12 +306,10 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
-      mbar_init(smem_u32(&sff_bar[s]), 1);
     }
     mbar_init(smem_u32(tfull_bar), 1);
     mbar_init(smem_u32(tempty_bar), EPW);
-    mbar_init(smem_u32(&drain_bar[0]), 1);
-    mbar_init(smem_u32(&drain_bar[1]), 1);
+    mbar_init(smem_u32(drain_bar), 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
@@ -374,17 +372,28 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     uint32_t acc_phase = 0;
     constexpr uint32_t idesc[2] = {idesc_mxf4(MG_BM, S::BN, 0), idesc_mxf4(MG_BM, S::BN, 2)};
     const uint64_t a0 = sdesc_kmajor_sw128(smem_u32(sA)), b0 = sdesc_kmajor_sw128(smem_u32(sB));
+    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
+    // A stage's scale slot in TMEM is free when the stage is: both wait for the MMAs of the round before.
     mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int, int kb, int s, uint32_t phase) {
       if (kb == 0 && !mbar_wait(smem_u32(tempty_bar), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
-      if (!mbar_wait(smem_u32(&sff_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       tc_fence_after();
       const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
       const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
+      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (2 * MG_SF_BYTES >> 4);
       if (one) {
+        const bool whole = 2 * kb + 1 < (int)p.katoms;
+        tc_cp_32x128b_warpx4(tsfa, sa);
+        tc_cp_32x128b_warpx4(tsfb, sb);
+        tc_cp_32x128b_warpx4(tsfb + 4, sb + (MG_SF_BYTES >> 4));
+        if (whole) {
+          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
+          tc_cp_32x128b_warpx4(tsfb + 8, sb + 32);
+          tc_cp_32x128b_warpx4(tsfb + 12, sb + (MG_SF_BYTES >> 4) + 32);
+        }
         mma_mxf4(0, a_d, b_d, idesc[0], tsfa, tsfb, kb != 0 ? 1u : 0u);
         mma_mxf4(0, a_d + 2, b_d + 2, idesc[1], tsfa, tsfb, 1u);
-        if (2 * kb + 1 < (int)p.katoms) {                           // a whole stage
+        if (whole) {
           mma_mxf4(0, a_d + 4, b_d + 4, idesc[0], tsfa + 4, tsfb + 8, 1u);
           mma_mxf4(0, a_d + 6, b_d + 6, idesc[1], tsfa + 4, tsfb + 8, 1u);
         }
@@ -393,31 +402,6 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
       }
       __syncwarp();
       if (kb + 1 == n_kblk) acc_phase ^= 1;
-      return true;
-    });
-  } else if (warp == COPIER) {
-    // ───────── scale copier ─────────
-    // Slot s is rewritten only after full[s] of the next round, posted after empty[s], which the
-    // MMA warp commits after the MMAs that read the slot.
-    const bool one = elect_one();
-    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
-    mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int, int kb, int s, uint32_t phase) {
-      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
-      tc_fence_after();
-      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
-      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (2 * MG_SF_BYTES >> 4);
-      if (one) {
-        tc_cp_32x128b_warpx4(tsfa, sa);
-        tc_cp_32x128b_warpx4(tsfb, sb);
-        tc_cp_32x128b_warpx4(tsfb + 4, sb + (MG_SF_BYTES >> 4));
-        if (2 * kb + 1 < (int)p.katoms) {
-          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
-          tc_cp_32x128b_warpx4(tsfb + 8, sb + 32);
-          tc_cp_32x128b_warpx4(tsfb + 12, sb + (MG_SF_BYTES >> 4) + 32);
-        }
-        tc_commit(smem_u32(&sff_bar[s]));
-      }
-      __syncwarp();
       return true;
     });
   } else {
@@ -449,12 +433,8 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
 
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
   if (warp == 1 && lane == 0) {
-    tc_commit(smem_u32(&drain_bar[0]));
-    mbar_wait(smem_u32(&drain_bar[0]), 0, nullptr, 0, MHMOE_DRAIN_NS);
-  }
-  if (warp == COPIER && lane == 0) {
-    tc_commit(smem_u32(&drain_bar[1]));
-    mbar_wait(smem_u32(&drain_bar[1]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+    tc_commit(smem_u32(drain_bar));
+    mbar_wait(smem_u32(drain_bar), 0, nullptr, 0, MHMOE_DRAIN_NS);
   }
   tc_fence_before();
   __syncthreads();
@@ -474,7 +454,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   pdl_wait();
   pdl_trigger();
   using S = FlatShape<BN>;
-  constexpr int STAGES = S::STAGES, EPW = S::EPW, COPIER = 2 + EPW, NACC = S::NACC;
+  constexpr int STAGES = S::STAGES, EPW = S::EPW, NACC = S::NACC;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -484,12 +464,11 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   uint8_t* sSTG = sSFB + STAGES * MG_SF_BYTES;
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(sSTG + EPW * 32 * MG_STG_FLAT);
   uint64_t* empty_bar = full_bar + STAGES;
-  uint64_t* sff_bar = empty_bar + STAGES;      // the stage's scales are in TMEM
-  uint64_t* tfull_bar = sff_bar + STAGES;      // [NACC]
+  uint64_t* tfull_bar = empty_bar + STAGES;    // [NACC]
   uint64_t* tempty_bar = tfull_bar + NACC;     // [NACC]
-  uint64_t* drain_bar = tempty_bar + NACC;     // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
-  static_assert((3 * STAGES + 2 * NACC + 2) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  uint64_t* drain_bar = tempty_bar + NACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  static_assert((2 * STAGES + 2 * NACC + 1) * 8 + 4 <= MG_MISC_BYTES, "barriers");
   static_assert(!SPLIT || BN * 128 * 4 <= STAGES * MG_A_BYTES, "partial sums lie over operand A's stages");
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
@@ -498,14 +477,12 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&full_bar[s]), 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
-      mbar_init(smem_u32(&sff_bar[s]), 1);
     }
     for (int a = 0; a < NACC; ++a) {
       mbar_init(smem_u32(&tfull_bar[a]), 1);
       mbar_init(smem_u32(&tempty_bar[a]), EPW);
     }
-    mbar_init(smem_u32(&drain_bar[0]), 1);
-    mbar_init(smem_u32(&drain_bar[1]), 1);
+    mbar_init(smem_u32(drain_bar), 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
@@ -572,18 +549,27 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     uint32_t acc = 0, acc_phase = 0;
     constexpr uint32_t idesc[2] = {idesc_mxf4(MG_BM, BN, 0), idesc_mxf4(MG_BM, BN, 2)};
     const uint64_t a0 = sdesc_kmajor_sw128(smem_u32(sA)), b0 = sdesc_kmajor_sw128(smem_u32(sB));
+    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
+    // A stage's scale slot in TMEM is free when the stage is: both wait for the MMAs of the round before.
     mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
       if (kb == kb0 && !mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout))
         return false;
       if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
-      if (!mbar_wait(smem_u32(&sff_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       tc_fence_after();
       const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
       const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8, d = acc * BN;
+      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (MG_SF_BYTES >> 4);
       if (one) {
+        const bool whole = 2 * kb + 1 < (int)p.katoms;
+        tc_cp_32x128b_warpx4(tsfa, sa);
+        tc_cp_32x128b_warpx4(tsfb, sb);
+        if (whole) {
+          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
+          tc_cp_32x128b_warpx4(tsfb + 4, sb + 32);
+        }
         mma_mxf4(d, a_d, b_d, idesc[0], tsfa, tsfb, kb != kb0 ? 1u : 0u);
         mma_mxf4(d, a_d + 2, b_d + 2, idesc[1], tsfa, tsfb, 1u);
-        if (2 * kb + 1 < (int)p.katoms) {                           // a whole stage
+        if (whole) {
           mma_mxf4(d, a_d + 4, b_d + 4, idesc[0], tsfa + 4, tsfb + 4, 1u);
           mma_mxf4(d, a_d + 6, b_d + 6, idesc[1], tsfa + 4, tsfb + 4, 1u);
         }
@@ -595,27 +581,6 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
         acc = 0;
         acc_phase ^= 1;
       }
-      return true;
-    });
-  } else if (warp == COPIER) {
-    // ───────── scale copier ─────────
-    const bool one = elect_one();
-    const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
-    mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
-      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
-      tc_fence_after();
-      const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
-      const uint64_t sa = sa0 + s * (MG_SF_BYTES >> 4), sb = sb0 + s * (MG_SF_BYTES >> 4);
-      if (one) {
-        tc_cp_32x128b_warpx4(tsfa, sa);
-        tc_cp_32x128b_warpx4(tsfb, sb);
-        if (2 * kb + 1 < (int)p.katoms) {
-          tc_cp_32x128b_warpx4(tsfa + 4, sa + 32);
-          tc_cp_32x128b_warpx4(tsfb + 4, sb + 32);
-        }
-        tc_commit(smem_u32(&sff_bar[s]));
-      }
-      __syncwarp();
       return true;
     });
   } else {
@@ -659,12 +624,8 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
 
   // Retire every tcgen05 op that was issued before TMEM is released (a formality unless a wait gave up).
   if (warp == 1 && lane == 0) {
-    tc_commit(smem_u32(&drain_bar[0]));
-    mbar_wait(smem_u32(&drain_bar[0]), 0, nullptr, 0, MHMOE_DRAIN_NS);
-  }
-  if (warp == COPIER && lane == 0) {
-    tc_commit(smem_u32(&drain_bar[1]));
-    mbar_wait(smem_u32(&drain_bar[1]), 0, nullptr, 0, MHMOE_DRAIN_NS);
+    tc_commit(smem_u32(drain_bar));
+    mbar_wait(smem_u32(drain_bar), 0, nullptr, 0, MHMOE_DRAIN_NS);
   }
   tc_fence_before();
   __syncthreads();
@@ -727,7 +688,10 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
 __device__ __forceinline__ int64_t clip(int64_t v, int64_t hi) { return v < 0 ? 0 : (v > hi ? hi : v); }
 
 struct MgGroup {
+  const void* x;              // activations, or with xq the tokens already in MXFP4
   int64_t x_stride, x_rows, R;
+  const uint8_t* xq;
+  const uint8_t* xsf;
   uint32_t cols, katoms;
   bool ceil, vec;
   const int64_t* offsets;
@@ -743,89 +707,106 @@ struct MgGroup {
   int* status;
 };
 
-// Block 0 lists the token tiles; every other warp quantises one sorted row.  Expert e's tiles
-// take the scale slots offsets[e] / slot_rows + e + 0, 1, ...: the sum of the rounded-up tile
-// counts before e is at most that, so no prefix sum has to come first.
+// The list of token tiles, by one block of 256 threads.  Expert e's tiles take the scale slots
+// offsets[e] / slot_rows + e + 0, 1, ...: the sum of the rounded-up tile counts before e is at most
+// that, so that the blocks that fill the slots need no prefix sum.
+__device__ __forceinline__ void mg_list_tiles(const MgGroup& p) {
+  __shared__ int wsum[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int base = 0;
+  bool bad = false;
+  for (int e0 = 0; e0 < p.n; e0 += 256) {
+    const int e = e0 + threadIdx.x;
+    int64_t a = 0;
+    int rows = 0;
+    if (e < p.n) {
+      const int64_t lo = p.offsets[e], hi = p.offsets[e + 1];
+      bad |= lo < 0 || lo > p.R || hi < lo || hi > p.R;
+      a = clip(lo, p.R);
+      rows = (int)max((int64_t)0, clip(hi, p.R) - a);
+    }
+    const int cnt = (rows + p.slot_rows - 1) / p.slot_rows;
+    int inc = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) wsum[warp] = inc;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int w = 0; w < 8; ++w) {
+      before += w < warp ? wsum[w] : 0;
+      all += wsum[w];
+    }
+    const int at = base + before + inc - cnt;
+    const int slot0 = (int)(a / p.slot_rows) + e;
+    for (int j = 0; j < cnt && at + j < p.max_tiles; ++j)
+      p.tiles[at + j] = make_int4(e, (int)a + j * p.slot_rows, min(p.slot_rows, rows - j * p.slot_rows), slot0 + j);
+    base += all;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) *p.n_tiles = min(base, p.max_tiles);
+  if (bad) record_error(p.status, MHMOE_ERR_ARGS);
+}
+
+// Where sorted row r goes and comes from.
+struct MgRow {
+  int64_t src;                // row of x, -1: a row of zeros (its id is outside x)
+  uint64_t sf;                // byte of its first scale word in MgGroup::sf
+  bool none;                  // no expert
+};
+__device__ __forceinline__ MgRow mg_row(const MgGroup& p, int64_t r, int e) {
+  MgRow w;
+  const int64_t a = clip(p.offsets[e], p.R);
+  w.none = a > r || clip(p.offsets[e + 1], p.R) <= r;       // before the first, behind the last (or offsets that decrease)
+  const int64_t tile = w.none ? 0 : (r - a) / p.slot_rows;
+  const int m = w.none ? 0 : (int)(r - a - tile * p.slot_rows);
+  w.sf = (uint64_t)(a / p.slot_rows + e + tile) * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
+  w.src = w.none ? -1 : (p.gather ? p.gather[r] : r);
+  if (!w.none && (w.src < 0 || w.src >= p.x_rows)) {
+    record_error(p.status, MHMOE_ERR_ARGS);
+    w.src = -1;
+  }
+  return w;
+}
+
+__device__ __forceinline__ void mg_clear_row(const MgGroup& p, int64_t r, int lane) {
+  uint8_t* o = p.y + r * p.y_pitch;              // elements of 2 or 4 bytes
+  for (int64_t i = lane * 2; i < p.y_row_bytes; i += 64) *reinterpret_cast<uint16_t*>(o + i) = 0;
+}
+
+// Block 0 lists the token tiles; every other warp quantises one sorted row.
 template <int DT>
-__global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>::T* __restrict__ x, const MgGroup p) {
+__global__ void __launch_bounds__(256) mx_group_kernel(const __grid_constant__ MgGroup p) {
   pdl_wait();
   pdl_trigger();
+  if (blockIdx.x == 0) return mg_list_tiles(p);
+  using T = typename MxType<DT>::T;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x == 0) {
-    __shared__ int wsum[8];
-    int base = 0;
-    bool bad = false;
-    for (int e0 = 0; e0 < p.n; e0 += 256) {
-      const int e = e0 + threadIdx.x;
-      int64_t a = 0;
-      int rows = 0;
-      if (e < p.n) {
-        const int64_t lo = p.offsets[e], hi = p.offsets[e + 1];
-        bad |= lo < 0 || lo > p.R || hi < lo || hi > p.R;
-        a = clip(lo, p.R);
-        rows = (int)max((int64_t)0, clip(hi, p.R) - a);
-      }
-      const int cnt = (rows + p.slot_rows - 1) / p.slot_rows;
-      int inc = cnt;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) wsum[warp] = inc;
-      __syncthreads();
-      int before = 0, all = 0;
-      for (int w = 0; w < 8; ++w) {
-        before += w < warp ? wsum[w] : 0;
-        all += wsum[w];
-      }
-      const int at = base + before + inc - cnt;
-      const int slot0 = (int)(a / p.slot_rows) + e;
-      for (int j = 0; j < cnt && at + j < p.max_tiles; ++j)
-        p.tiles[at + j] = make_int4(e, (int)a + j * p.slot_rows, min(p.slot_rows, rows - j * p.slot_rows), slot0 + j);
-      base += all;
-      __syncthreads();
-    }
-    if (threadIdx.x == 0) *p.n_tiles = min(base, p.max_tiles);
-    if (bad) record_error(p.status, MHMOE_ERR_ARGS);
-    return;
-  }
   const int64_t r = (int64_t)(blockIdx.x - 1) * 8 + warp;
   if (r >= p.R) return;
-  // the last expert whose first row is at or before r
-  int e = 0;
-  int64_t a = 0;
-  bool none = clip(p.offsets[0], p.R) > r || clip(p.offsets[p.n], p.R) <= r;
-  if (!none) {
-    int len = p.n;
-    while (len > 1) {
-      const int step = (len + 31) / 32, i = e + lane * step;
-      const bool le = lane * step < len && clip(p.offsets[i], p.R) <= r;
-      const int k = max(__popc(__ballot_sync(0xffffffffu, le)), 1) - 1;
-      e += k * step;
-      len = min(step, len - k * step);
-    }
-    a = clip(p.offsets[e], p.R);
-    none = a > r;                                // only with offsets that decrease
+  // the last expert whose first row is at or before r, 32 candidates a step
+  int e = 0, len = p.n;
+  while (len > 1) {
+    const int step = (len + 31) / 32, i = e + lane * step;
+    const bool le = lane * step < len && clip(p.offsets[i], p.R) <= r;
+    const int k = max(__popc(__ballot_sync(0xffffffffu, le)), 1) - 1;
+    e += k * step;
+    len = min(step, len - k * step);
   }
-  if (none) {
-    if (p.zero_tail) {
-      uint8_t* o = p.y + r * p.y_pitch;          // elements of 2 or 4 bytes
-      for (int64_t i = lane * 2; i < p.y_row_bytes; i += 64) *reinterpret_cast<uint16_t*>(o + i) = 0;
-    }
+  const MgRow w = mg_row(p, r, e);
+  if (w.none) {
+    if (p.zero_tail) mg_clear_row(p, r, lane);
     return;
   }
-  const int m = (int)(r - a) % p.slot_rows;
-  const int64_t slot = a / p.slot_rows + e + (r - a) / p.slot_rows;
-  int64_t src = p.gather ? p.gather[r] : r;
-  const bool ok = src >= 0 && src < p.x_rows;
-  if (!ok && lane == 0) record_error(p.status, MHMOE_ERR_ARGS);
-  const typename MxType<DT>::T* xr = x + (ok ? src : 0) * p.x_stride;
+  const bool ok = w.src >= 0;
+  const T* xr = static_cast<const T*>(p.x) + (ok ? w.src : 0) * p.x_stride;
   uint8_t* d = p.data + r * (int64_t)p.katoms * 64;
-  uint8_t* s = p.sf + (uint64_t)slot * p.katoms * 512 + (m & 31) * 16 + (m >> 5) * 4;
+  uint8_t* s = p.sf + w.sf;
 #pragma unroll 2
   for (uint32_t c0 = lane * 16; c0 < (p.katoms + 3) / 4 * 512; c0 += 512) {
-    MxRaw16<typename MxType<DT>::T> v;
+    MxRaw16<T> v;
     const bool live = ok && c0 < p.cols;
     v.load(xr + c0, live && p.vec && c0 + 16 <= p.cols, live ? (int)min(16u, p.cols - c0) : 0);
     uint2 code;
@@ -837,6 +818,58 @@ __global__ void __launch_bounds__(256) mx_group_kernel(const typename MxType<DT>
   }
 }
 
+// The same from tokens that are quantised already (once a token instead of once a row): every other
+// warp copies MG_COPY_ROWS sorted rows, all their loads in flight together.
+constexpr int MG_COPY_ROWS = 8;
+__global__ void __launch_bounds__(256) mx_group_copy_kernel(const __grid_constant__ MgGroup p, const FastDiv katoms) {
+  pdl_wait();
+  pdl_trigger();
+  if (blockIdx.x == 0) return mg_list_tiles(p);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = ((int64_t)(blockIdx.x - 1) * 8 + warp) * MG_COPY_ROWS;
+  if (r0 >= p.R) return;
+  const int rows = (int)min((int64_t)MG_COPY_ROWS, p.R - r0);
+  // one lane a row: the last expert whose first row is at or before it
+  MgRow w{-1, 0, true};
+  if (lane < rows) {
+    int e = 0, hi = p.n - 1;
+    while (e < hi) {
+      const int mid = (e + hi + 1) >> 1;
+      if (clip(p.offsets[mid], p.R) <= r0 + lane) e = mid;
+      else hi = mid - 1;
+    }
+    w = mg_row(p, r0 + lane, e);
+  }
+  const uint32_t n16 = katoms.d * 4;               // 16-B chunks of a row
+  for (uint32_t i = lane; i < (n16 + 31) / 32 * 32; i += 32) {
+    uint4 v[MG_COPY_ROWS];
+#pragma unroll
+    for (int k = 0; k < MG_COPY_ROWS; ++k) {
+      const int64_t src = __shfl_sync(0xffffffffu, w.src, k);
+      v[k] = src >= 0 && i < n16 ? __ldg(reinterpret_cast<const uint4*>(p.xq + src * katoms.d * 64) + i)
+                                 : make_uint4(0, 0, 0, 0);
+    }
+    const unsigned none = __ballot_sync(0xffffffffu, w.none);
+#pragma unroll
+    for (int k = 0; k < MG_COPY_ROWS; ++k)
+      if (!(none >> k & 1) && i < n16) reinterpret_cast<uint4*>(p.data + (r0 + k) * (int64_t)katoms.d * 64)[i] = v[k];
+  }
+  // scale words: row k, atom a
+  for (uint32_t i = lane; i < (MG_COPY_ROWS * katoms.d + 31) / 32 * 32; i += 32) {
+    const uint32_t k = katoms.div(i), a = i - k * katoms.d;
+    const int from = (int)min(k, (uint32_t)MG_COPY_ROWS - 1);
+    const int64_t src = __shfl_sync(0xffffffffu, w.src, from);
+    const uint64_t at = __shfl_sync(0xffffffffu, w.sf, from);
+    const bool none = __shfl_sync(0xffffffffu, (int)w.none, from) != 0;
+    if (k < MG_COPY_ROWS && !none)
+      *reinterpret_cast<uint32_t*>(p.sf + at + a * 512) =
+          src >= 0 ? __ldg(reinterpret_cast<const uint32_t*>(p.xsf + mx_sf_offset(src, a * 4, katoms.d))) : 0u;
+  }
+  if (p.zero_tail)
+    for (unsigned none = __ballot_sync(0xffffffffu, w.none && lane < rows); none; none &= none - 1)
+      mg_clear_row(p, r0 + __ffs(none) - 1, lane);
+}
+
 // ───────────────────────────── launch ─────────────────────────────
 
 struct MgPlan {
@@ -844,12 +877,13 @@ struct MgPlan {
   int bn, slot_rows, split;
   int64_t tiles, slots;       // token tiles at most; scale slots
   int n_wt;
+  bool once;                  // quantise the tokens first, then copy their rows
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Orientation, tile and split by the sizes alone.
-MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
+MgPlan mg_plan(int64_t x_rows, int64_t R, int n, int N, int64_t katoms, bool grouped) {
   const int sms = num_sms();
   MgPlan g;
   const int64_t avg = grouped ? ceil_div(R, n) : R;
@@ -871,6 +905,9 @@ MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
   g.tiles = tiles_of(g.slot_rows);
   g.slots = grouped ? R / g.slot_rows + n + 1 : g.tiles;
   g.n_wt = (int)ceil_div(N, g.flat ? 128 : 256);
+  // Copying a row costs a third of quantising it, a launch more about 2 us (top-8 of 128 experts, 1024
+  // columns: 8192 rows 16.1 us quantised each, 17.7 copied; 32768 rows 38.3 and 30.8).
+  g.once = grouped && R >= 2 * x_rows && R >= 16384;
   g.split = 1;
   const int64_t n_kblk = ceil_div(katoms, 2);
   while (g.flat && g.split < 8 && g.tiles * g.n_wt * g.split * 2 <= sms && g.split * 2 <= n_kblk) g.split *= 2;
@@ -878,16 +915,18 @@ MgPlan mg_plan(int64_t R, int n, int N, int64_t katoms, bool grouped) {
 }
 
 struct MgScratch {
-  size_t data, sf, tiles, count, bytes;
+  size_t data, sf, tiles, count, tok, tok_sf, bytes;
 };
-MgScratch mg_scratch(const MgPlan& g, int64_t R, int64_t katoms, bool grouped) {
+MgScratch mg_scratch(const MgPlan& g, int64_t x_rows, int64_t R, int64_t katoms, bool grouped) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   MgScratch s;
   s.data = 0;
   s.sf = up((size_t)R * katoms * 64);
   s.tiles = s.sf + up((size_t)(grouped ? g.slots : ceil_div(R, 128)) * katoms * 512);
   s.count = s.tiles + (grouped ? up((size_t)g.tiles * sizeof(int4)) : 0);
-  s.bytes = s.count + (grouped ? 256 : 0);
+  s.tok = s.count + (grouped ? 256 : 0);
+  s.tok_sf = s.tok + (g.once ? up((size_t)x_rows * katoms * 64) : 0);
+  s.bytes = s.tok_sf + (g.once ? (size_t)ceil_div(x_rows, 128) * katoms * 512 : 0);
   return s;
 }
 
@@ -956,15 +995,15 @@ cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
 size_t mx_product_workspace_bytes(int64_t x_rows, int64_t R, int n, int N, int cols, bool grouped) {
   const int64_t katoms = mx_padded_cols(cols) / 128;
   if (R == 0) return 0;
-  return mg_scratch(mg_plan(R, n, N, katoms, grouped), R, katoms, grouped).bytes;
+  return mg_scratch(mg_plan(x_rows, R, n, N, katoms, grouped), x_rows, R, katoms, grouped).bytes;
 }
 
 int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t* cerr) {
   const int64_t katoms = mx_padded_cols(p.cols) / 128;
   const bool grouped = p.offsets != nullptr;
-  const MgPlan g = mg_plan(p.R, p.n, p.N, katoms, grouped);
+  const MgPlan g = mg_plan(p.x_rows, p.R, p.n, p.N, katoms, grouped);
   if (g.tiles * g.n_wt >= (int64_t)1 << 30) return MHMOE_ERR_CAPACITY;
-  const MgScratch ws = mg_scratch(g, p.R, katoms, grouped);
+  const MgScratch ws = mg_scratch(g, p.x_rows, p.R, katoms, grouped);
   uint8_t* base = static_cast<uint8_t*>(workspace);
   const int64_t y_esz = p.y_dtype == DT_F32 ? 4 : 2, n_out = p.act ? p.N / 2 : p.N;
   const uint8_t* data = p.xq;
@@ -994,13 +1033,21 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
     q.y_pitch = p.y_stride * y_esz;
     q.zero_tail = p.zero_tail;
     q.status = p.status;
-    const unsigned grid = (unsigned)(1 + ceil_div(p.R, 8));
-    if (p.x_dtype == DT_F32)
-      *cerr = launch_pdl(mx_group_kernel<DT_F32>, dim3(grid), dim3(256), 0, st, static_cast<const float*>(p.x), q);
-    else if (p.x_dtype == DT_BF16)
-      *cerr = launch_pdl(mx_group_kernel<DT_BF16>, dim3(grid), dim3(256), 0, st, static_cast<const __nv_bfloat16*>(p.x), q);
-    else
-      *cerr = launch_pdl(mx_group_kernel<DT_F16>, dim3(grid), dim3(256), 0, st, static_cast<const __half*>(p.x), q);
+    q.x = p.x;
+    if (g.once) {
+      q.xq = base + ws.tok;
+      q.xsf = base + ws.tok_sf;
+      *cerr = launch_mx_quantize(p.x, p.x_dtype, 0, p.x_stride, 1, p.x_rows, p.cols, p.ceil, base + ws.tok,
+                                 base + ws.tok_sf, st);
+      if (*cerr == cudaSuccess)
+        *cerr = launch_pdl(mx_group_copy_kernel, dim3((unsigned)(1 + ceil_div(p.R, 8 * MG_COPY_ROWS))), dim3(256), 0, st,
+                           q, FastDiv((uint32_t)katoms));
+    } else {
+      const dim3 grid((unsigned)(1 + ceil_div(p.R, 8)));
+      *cerr = p.x_dtype == DT_F32    ? launch_pdl(mx_group_kernel<DT_F32>, grid, dim3(256), 0, st, q)
+              : p.x_dtype == DT_BF16 ? launch_pdl(mx_group_kernel<DT_BF16>, grid, dim3(256), 0, st, q)
+                                     : launch_pdl(mx_group_kernel<DT_F16>, grid, dim3(256), 0, st, q);
+    }
     data = q.data;
     a.sf_tok = q.sf;
     a.tiles = q.tiles;
