@@ -176,12 +176,18 @@ __device__ __forceinline__ void sort_keys(unsigned (&k)[N]) {
           }
 }
 
-// Bytes of shared memory a warp needs: 64-bit keys and group scores of a row done again, which
-// also hold the lanes' sorted keys (32 (NPL + 1) words <= 8 E + 512).
-__host__ __device__ constexpr int fwd_scratch_bytes(int E) { return 8 * E + 512; }
+// Bytes of shared memory a warp needs: the lanes' sorted keys of its rows (NPL and a 0 behind them),
+// over which a row that is done again puts its 64-bit keys and group scores; and a row's keys by
+// expert, to walk groups in.
+__host__ __device__ constexpr int fwd_scratch_bytes(int E, int npl, int rpw, bool grouped) {
+  const int lists = rpw * (npl + 1) * 128, again = 8 * E + 512;
+  return (lists > again ? lists : again) + (grouped ? (4 * E + 7) / 8 * 8 : 0);
+}
 
-// A warp takes `rpw` consecutive rows one after another; what follows the selection (scores of the
-// chosen, normalisation, stores) is done for all of them at once, seg = 32 / rpw >= K lanes a row.
+// A warp takes RPW consecutive rows: scores, keys and sorting one row after another, the selection's
+// rounds for all of them together (a round is a chain of a warp-wide maximum and a load, which one
+// row alone leaves waiting), and what follows (scores of the chosen, normalisation, stores) for all
+// at once, 32 / RPW >= K lanes a row.
 //
 // Lane l holds experts [l * NPL, (l + 1) * NPL) of the row in registers.  A key is the order-preserving map of
 // the candidate's fp32 value with its low bits replaced by the complement of the expert's id:
@@ -196,10 +202,9 @@ __host__ __device__ constexpr int fwd_scratch_bytes(int E) { return 8 * E + 512;
 // argument and exponential), a sigmoid by less than 2^-21, the sum with the bias by half a unit
 // of 2^-23; a difference of two by twice that, of two group sums by four times.  Logits
 // themselves (no bias) are exact: 16-bit ones fit above the id bits, so their keys are too.
-template <int DT, int NPL>
-__global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 : 4)
-    route_experts_kernel(const __grid_constant__ RouteArgs a, bool vec, unsigned per_magic, int rpw,
-                         float* __restrict__ weights, int64_t* __restrict__ idx, float* __restrict__ saved) {
+template <int DT, int NPL, int RPW, bool GROUPED>
+__global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 4)
+    route_experts_kernel(const __grid_constant__ RouteArgs a, bool vec, unsigned per_magic, float* __restrict__ weights, int64_t* __restrict__ idx, float* __restrict__ saved) {
   pdl_wait();
   pdl_trigger();
   using T = typename MxType<DT>::T;
@@ -207,28 +212,50 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
   constexpr float LOG2E = 1.44269504f;
   extern __shared__ double smd[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned rows = (unsigned)(a.H * a.S), row0 = (blockIdx.x * RE_WARPS + warp) * (unsigned)rpw;
+  constexpr int SEG = 32 / RPW;
+  const unsigned rows = (unsigned)(a.H * a.S), row0 = (blockIdx.x * RE_WARPS + warp) * RPW;
   if (row0 >= rows) return;
-  const int n_rows = (int)min((unsigned)rpw, rows - row0), seg = 32 / rpw;
+  const int n_rows = (int)min((unsigned)RPW, rows - row0), mine_r = lane / SEG, rank = lane % SEG;
   const int E = a.E, K = a.K, e0 = lane * NPL, G = a.groups;
-  const bool grouped = a.keep < G, exact = DT != DT_F32 && !a.bias;
-  double* scratch = smd + (size_t)warp * (fwd_scratch_bytes(E) / 8);
-  // of this lane's choice (row row0 + lane / seg, rank lane % seg)
+  const bool exact = DT != DT_F32 && !a.bias;
+  const int bytes = fwd_scratch_bytes(E, NPL, RPW, GROUPED);
+  double* scratch = smd + (size_t)warp * (bytes / 8);
+  unsigned* lists = reinterpret_cast<unsigned*>(scratch);         // [RPW][NPL + 1][32]
+  unsigned* words = lists + bytes / 4 - (E + 1) / 2 * 2;          // [E], with groups
+  float b[NPL];                                                   // the head's biases
+  bool b_odd = false;                                             // one of them is no number
+  // of this lane's choice (row row0 + mine_r, the rank-th)
   unsigned mine_key = 0, extra = 0;
   float m_l = 0.f, sum_l = 1.f, tol_l = 0x1p-20f;
   bool close = false;
   unsigned h = row0 / (unsigned)a.S, s = row0 - h * (unsigned)a.S;
+  // a row's logits are loaded while the row before is worked on
+  float ahead[NPL];
+  auto fetch = [&](unsigned fh, unsigned fs) {
+    load_chunk<T, NPL>(static_cast<const T*>(a.logits) + fh * a.stride_h + fs * a.stride_s, e0, E, vec, -INFINITY, ahead);
+  };
+  fetch(h, s);
   for (int r = 0; r < n_rows; ++r, ++s) {
     if (s == (unsigned)a.S) {
       s = 0;
       ++h;
     }
-    if (a.token_mask && !a.token_mask[h * a.mask_stride_h + s]) continue;
-    const bool mine_row = lane / seg == r;
-    const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
-    const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
+    if (a.bias && (r == 0 || s == 0)) {
+      load_chunk<float, NPL>(a.bias + (int64_t)h * E, e0, E, vec, 0.f, b);
+      float probe = 0.f;
+#pragma unroll
+      for (int j = 0; j < NPL; ++j) probe = fmaf(b[j], 0.f, probe);
+      b_odd = !(probe == 0.f);
+    }
     float x[NPL];
-    load_chunk<T, NPL>(lg, e0, E, vec, -INFINITY, x);
+#pragma unroll
+    for (int j = 0; j < NPL; ++j) x[j] = ahead[j];
+    if (r + 1 < n_rows) fetch(s + 1 == (unsigned)a.S ? h + 1 : h, s + 1 == (unsigned)a.S ? 0u : s + 1);
+    unsigned* list = lists + r * (NPL + 1) * 32 + lane;
+    list[0] = 0;                                                  // for a row without a choice
+    if (a.token_mask && !a.token_mask[h * a.mask_stride_h + s]) continue;
+    const bool mine_row = mine_r == r;
+    const bool bias = a.bias != nullptr;
     // infinities and NaN make a product with 0 that is not 0; lanes that reach over E count too
     float probe = 0.f;
 #pragma unroll
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
       if (m == -INFINITY) continue;                               // no expert is left
     }
     unsigned key[NPL];
-    if (bias || grouped || a.score_func == 0) {
+    if (bias || GROUPED || a.score_func == 0) {
       float v[NPL];
       if (a.score_func == 0) {
         float sum = 0.f;
@@ -266,7 +293,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
           sum_l = sum;
         }
         tol0 = smax * 0x1p-17f;
-        if (bias || grouped) {
+        if (bias || GROUPED) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j) v[j] *= smax;
         }
@@ -274,41 +301,31 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
 #pragma unroll
         for (int j = 0; j < NPL; ++j) v[j] = rcp_approx(1.f + ex2_approx(x[j] * -LOG2E));
       }
-      if (bias || grouped) {
+      if (bias || GROUPED) {
         if (bias) {
-          float b[NPL];
-          load_chunk<float, NPL>(bias, e0, E, vec, 0.f, b);
 #pragma unroll
           for (int j = 0; j < NPL; ++j) v[j] += b[j];
         }
 #pragma unroll
         for (int j = 0; j < NPL; ++j) key[j] = order_key(v[j]);
         // experts without a number: masked ones (a bias may be -inf too) and NaN
-        bool odd = special;
-        if (bias) {
-          float pv = 0.f;
-#pragma unroll
-          for (int j = 0; j < NPL; ++j) pv = fmaf(v[j], 0.f, pv);
-          odd |= !(pv == 0.f);
-        }
-        if (odd) {
+        if (special || b_odd) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j) {
             if (v[j] != v[j]) key[j] = order_key(-FLT_MAX);
-            if (x[j] == -INFINITY || (bias && e0 + j < E && bias[e0 + j] == -INFINITY)) key[j] = 0;
+            if (x[j] == -INFINITY || (bias && b[j] == -INFINITY)) key[j] = 0;
           }
         }
       }
     }
     unsigned long long kept = ~0ull;
-    if (grouped) {
+    if constexpr (GROUPED) {
       // two best of every group: 32 / G lanes (a power of two) walk a group in shared memory
       const int per = E / G;
-      unsigned* sv = reinterpret_cast<unsigned*>(scratch);
       __syncwarp();
 #pragma unroll
       for (int j = 0; j < NPL; ++j)
-        if (e0 + j < E) sv[e0 + j] = key[j];
+        if (e0 + j < E) words[e0 + j] = key[j];
       __syncwarp();
       const int lanes = G > 16 ? 1 : G > 8 ? 2 : G > 4 ? 4 : G > 2 ? 8 : 16;
       unsigned gk[2];
@@ -319,7 +336,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
         unsigned b1 = 0, b2 = 0;
         if (g < G)
           for (int i = lane & (lanes - 1); i < per; i += lanes) {
-            const unsigned k = sv[g * per + i];
+            const unsigned k = words[g * per + i];
             b2 = max(b2, min(b1, k));
             b1 = max(b1, k);
           }
@@ -360,7 +377,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
         for (int j = 0; j < NPL; ++j) key[j] = order_key(x[j] + 0.f);        // -0 ranks as 0
       }
     }
-    if (grouped) {
+    if constexpr (GROUPED) {
       const int g0 = (int)((e0 * per_magic) >> 20), per = E / G;
       if (per >= NPL) {                                           // a lane's experts lie in two groups at most
         const bool in0 = kept >> (g0 & 63) & 1ull, in1 = kept >> ((g0 + 1) & 63) & 1ull;
@@ -377,69 +394,78 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
 #pragma unroll
     for (int j = 0; j < NPL; ++j) key[j] = (key[j] & high) | (ID - e0 - j);
     sort_keys(key);
-    unsigned* list = reinterpret_cast<unsigned*>(scratch) + lane;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) list[j * 32] = key[j];
     list[NPL * 32] = 0;
-    // K rounds, and one more that shows the first one left out; what is left when nothing is, are
-    // bare ids, and 0 behind them, which is not taken off
-    unsigned top = key[0];
-    int slot = r * seg - lane;
-#pragma unroll 4
-    for (int k = 0; k < K; ++k, ++slot) {
-      const unsigned best = __reduce_max_sync(FULL, top);
-      mine_key = slot == 0 ? best : mine_key;
-      list += top == best && best ? 32 : 0;
-      top = *list;
-    }
-    if (!exact) {
-      const unsigned best = __reduce_max_sync(FULL, top);
-      extra = mine_row && best > ID ? best : extra;
-    }
     if (mine_row) tol_l = tol0;
   }
 
+  // K rounds, and one more that shows the first one left out; what is left when nothing is, are bare
+  // ids, and 0 behind them, which is not taken off
+  unsigned at[RPW], top[RPW];
+#pragma unroll
+  for (int r = 0; r < RPW; ++r) {
+    at[r] = r * (NPL + 1) * 32 + lane;
+    top[r] = r < n_rows ? lists[at[r]] : 0u;
+  }
+#pragma unroll(RPW == 1 ? 4 : 2)
+  for (int k = 0; k < K; ++k) {
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+      const unsigned best = __reduce_max_sync(FULL, top[r]);
+      mine_key = lane == r * SEG + k ? best : mine_key;
+      at[r] += top[r] == best && best ? 32 : 0;
+      top[r] = r < n_rows ? lists[at[r]] : 0u;
+    }
+  }
+  if (!exact) {
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+      const unsigned best = __reduce_max_sync(FULL, top[r]);
+      extra = mine_r == r && best > ID ? best : extra;
+    }
+  }
+
   // each lane its own choice
-  const int rank = lane % seg;
-  const unsigned row = row0 + lane / seg;
-  const bool live = lane / seg < n_rows && rank < K;
+  const unsigned row = row0 + mine_r;
+  const bool live = mine_r < n_rows && rank < K;
   h = row / (unsigned)a.S;
   s = row - h * (unsigned)a.S;
   const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
   const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
   int mine = mine_key > ID ? (int)(ID - (mine_key & ID)) : -1;
-  float x = 0.f, p = 0.f, b = 0.f;
+  float x = 0.f, p = 0.f, b_mine = 0.f;
   auto score = [&] {
     p = 0.f;
     if (mine >= 0) {
       x = mx_to_f32(lg[mine]);
-      p = a.score_func == 0 ? __fdiv_rn(expf(x - m_l), sum_l) : __fdiv_rn(1.f, 1.f + expf(-x));
+      p = a.score_func == 0 ? __fdividef(expf(x - m_l), sum_l) : __fdividef(1.f, 1.f + expf(-x));
     }
   };
   score();
   if (!exact) {
-    if (bias && mine >= 0) b = bias[mine];
-    const float v = bias ? p + b : x;
+    if (bias && mine >= 0) b_mine = bias[mine];
+    const float v = bias ? p + b_mine : x;
     const float tol = bias ? tol_l + 0x1p-22f * fabsf(v) : 0.f;
-    const float v1 = __shfl_down_sync(FULL, v, 1), x1 = __shfl_down_sync(FULL, x, 1), b1 = __shfl_down_sync(FULL, b, 1);
+    const float v1 = __shfl_down_sync(FULL, v, 1), x1 = __shfl_down_sync(FULL, x, 1), b1 = __shfl_down_sync(FULL, b_mine, 1);
     const bool next = __shfl_down_sync(FULL, mine, 1) >= 0;
     if (mine >= 0) {
       if (rank + 1 < K) {
-        if (next) close |= !(v - v1 > tol) && !(x == x1 && b == b1);
+        if (next) close |= !(v - v1 > tol) && !(x == x1 && b_mine == b1);
       } else if (extra) {
         close |= !(v - key_value(extra | ID) > tol);
       }
     }
   }
   for (unsigned again = __ballot_sync(FULL, close && live); again;) {
-    const int r = (__ffs(again) - 1) / seg;
-    again &= seg == 32 ? 0u : ~(((1u << seg) - 1u) << (r * seg));
+    const int r = (__ffs(again) - 1) / SEG;
+    again &= SEG == 32 ? 0u : ~(((1u << (SEG & 31)) - 1u) << (r * SEG));
     __syncwarp();
     const unsigned rr = row0 + r, hr = rr / (unsigned)a.S;
     const int id = select_row64<T>(a, static_cast<const T*>(a.logits) + hr * a.stride_h + (rr - hr * a.S) * a.stride_s,
                                    a.bias ? a.bias + (int64_t)hr * E : nullptr, scratch, lane);
     const int got = __shfl_sync(FULL, id, rank);
-    if (lane / seg == r) {
+    if (mine_r == r) {
       mine = got;
       score();
     }
@@ -447,8 +473,9 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 10 : NPL <= 16 ? 6 :
   float w = p;
   if (a.route_norm) {
     float n = p;
-    for (int o = seg / 2; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
-    w = __fdiv_rn(p, n != n ? n : fmaxf(n, a.norm_eps));
+    #pragma unroll
+    for (int o = SEG / 2; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
+    w = __fdividef(p, n != n ? n : fmaxf(n, a.norm_eps));
   }
   if (live) {
     const int64_t o = (int64_t)row * K + rank;
@@ -570,30 +597,46 @@ bool chunks_aligned(const void* p, int64_t stride_h, int64_t stride_s, int E, in
          stride_s * esz % unit == 0;
 }
 
-// Rows a warp takes: as many as have K lanes each, while 16 warps a SM are left.
+// Rows a warp takes, up to 4: as many as have K lanes each, while 16 warps a SM are left.
 int rows_per_warp(int64_t rows, int K) {
   int rpw = 1;
-  while (2 * rpw * K <= 32 && rpw < 8 && rows >= (int64_t)num_sms() * 16 * rpw * 2) rpw *= 2;
+  while (2 * rpw * K <= 32 && rpw < 4 && rows >= (int64_t)num_sms() * 16 * rpw * 2) rpw *= 2;
   return rpw;
 }
 
-template <int DT, int NPL>
+template <int DT, int NPL, int RPW, bool GROUPED>
 cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
   const int64_t rows = (int64_t)a.H * a.S;
-  const int rpw = rows_per_warp(rows, a.K);
-  const unsigned grid = (unsigned)((rows + RE_WARPS * rpw - 1) / (RE_WARPS * rpw));
-  const size_t smem = (size_t)RE_WARPS * fwd_scratch_bytes(a.E);
+  const unsigned grid = (unsigned)((rows + RE_WARPS * RPW - 1) / (RE_WARPS * RPW));
+  const size_t smem = (size_t)RE_WARPS * fwd_scratch_bytes(a.E, NPL, RPW, GROUPED);
+  auto kernel = route_experts_kernel<DT, NPL, RPW, GROUPED>;
   if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(route_experts_kernel<DT, NPL>,
-                                               cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
   }
   const bool vec = chunks_aligned(a.logits, a.stride_h, a.stride_s, a.E, DT == DT_F32 ? 4 : 2, NPL) &&
                    (!a.bias || chunks_aligned(a.bias, a.E, 0, a.E, 4, NPL));
   // e / per = e * ceil(2^20 / per) >> 20 for e < 1024
   const unsigned per = (unsigned)(a.E / a.groups), magic = ((1u << 20) + per - 1) / per;
-  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL>), grid, RE_WARPS * 32, smem, st, a, vec, magic, rpw, weights, idx, saved);
+  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL, RPW, GROUPED>), grid, RE_WARPS * 32, smem, st, a, vec, magic, weights,
+                   idx, saved);
   return cudaGetLastError();
+}
+
+template <int DT, int NPL, bool GROUPED>
+cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
+  if constexpr (NPL <= 8) {
+    const int rpw = rows_per_warp((int64_t)a.H * a.S, a.K);
+    if (rpw == 4) return run_fwd<DT, NPL, 4, GROUPED>(a, weights, idx, saved, st);
+    if (rpw == 2) return run_fwd<DT, NPL, 2, GROUPED>(a, weights, idx, saved, st);
+  }
+  return run_fwd<DT, NPL, 1, GROUPED>(a, weights, idx, saved, st);
+}
+
+template <int DT, int NPL>
+cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
+  return a.keep < a.groups ? run_fwd<DT, NPL, true>(a, weights, idx, saved, st)
+                           : run_fwd<DT, NPL, false>(a, weights, idx, saved, st);
 }
 
 template <int DT, int NPL>
