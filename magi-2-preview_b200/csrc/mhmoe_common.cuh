@@ -130,6 +130,13 @@ __device__ __forceinline__ bool flag_wait_geq(const int* flag, int expected, int
   }
 }
 
+// 32 bytes to 32-byte aligned global memory in one store.
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // y[0..8) += v (8 bf16 as 4 packed pairs), one 16-B vector atomic in L2 (16-B aligned).
 __device__ __forceinline__ void red_add_bf16x8(void* y, const uint32_t (&v)[4]) {
   asm volatile("red.global.add.noftz.v4.bf16x2 [%0], {%1, %2, %3, %4};" ::"l"(y), "r"(v[0]), "r"(v[1]), "r"(v[2]),

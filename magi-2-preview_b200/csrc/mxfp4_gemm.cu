@@ -73,7 +73,7 @@ struct MgParams {
   void* y;
   int y_dtype;
   int64_t y_stride;
-  bool y_vec;                 // 16-B stores are possible
+  bool y_vec, y_vec32;        // 16-B, 32-B stores are possible
   int* status;
   uint64_t timeout_ns;
 };
@@ -83,20 +83,24 @@ struct MgTile {
   int64_t row0, slot;
 };
 
+// A tile's entry is fetched a tile ahead and taken apart only when it is used, so that nothing waits
+// for the load in between.
+__device__ __forceinline__ int4 mg_fetch(const MgParams& p, int tt) {
+  return p.tiles ? __ldg(p.tiles + tt) : make_int4(0, 0, tt, 0);
+}
 template <int SLOT>
-__device__ __forceinline__ MgTile mg_tile(const MgParams& p, int tt) {
+__device__ __forceinline__ MgTile mg_tile(const MgParams& p, const int4& v) {
   MgTile t;
   if (p.tiles) {
-    const int4 v = __ldg(p.tiles + tt);
     t.e = v.x;
     t.row0 = v.y;
     t.rows = v.z;
     t.slot = v.w;
   } else {
     t.e = 0;
-    t.row0 = (int64_t)tt * SLOT;
+    t.row0 = (int64_t)v.z * SLOT;
     t.rows = (int)min((int64_t)SLOT, p.R - t.row0);
-    t.slot = tt;
+    t.slot = v.z;
   }
   return t;
 }
@@ -155,13 +159,16 @@ __device__ __forceinline__ void mg_store_rows(const MgParams& p, const uint8_t* 
   }
 }
 
-// Wide epilogue: 32 token rows (one a thread) x 64 accumulator columns from weight row col0.
+// Wide epilogue: 32 token rows (one a thread) x 64 accumulator columns from weight row col0.  A thread
+// stores its row's outputs as whole sectors of 32 B, or, where y's rows do not start on those, through
+// the staging.
 template <int OUT, bool SWIGLU>
 __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile& t, uint32_t (&r)[64], int col0,
                                                  int m0, int lane, uint8_t* stg) {
   constexpr int ESZ = OUT == DT_F32 ? 4 : 2;
-  constexpr int PER = MG_STG_WIDE / ESZ;            // outputs of a staging row
+  constexpr int PER = 32 / ESZ;                     // outputs of a sector, or of a staging row
   constexpr int ACC = SWIGLU ? 2 * PER : PER;       // accumulator columns behind them
+  static_assert(MG_STG_WIDE == 32, "a sector a row");
   const int n_out = SWIGLU ? p.N / 2 : p.N;
   if (p.bias) {
     const float* bias = p.bias + (int64_t)t.e * p.N + col0;
@@ -169,36 +176,40 @@ __device__ __forceinline__ void mg_wide_epilogue(const MgParams& p, const MgTile
     for (int i = 0; i < 64; ++i)
       if (col0 + i < p.N) r[i] = __float_as_uint(__uint_as_float(r[i]) + __ldg(bias + i));
   }
+  const bool live = m0 + lane < t.rows;
   float rw = 1.f;
-  if (p.row_weights && m0 + lane < t.rows) rw = __ldg(p.row_weights + t.row0 + m0 + lane);
+  if (p.row_weights && live) rw = __ldg(p.row_weights + t.row0 + m0 + lane);
+  const int o0 = SWIGLU ? col0 / 2 : col0;
+  uint8_t* dst = static_cast<uint8_t*>(p.y) + ((t.row0 + m0 + lane) * p.y_stride + o0) * ESZ;
 #pragma unroll
   for (int c = 0; c < 64 / ACC; ++c) {
     float v[PER];
+    const uint32_t* rc = r + c * ACC;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      if constexpr (SWIGLU)
-        v[i] = mx_swiglu7(__uint_as_float(r[c * ACC + 2 * i]), __uint_as_float(r[c * ACC + 2 * i + 1]));
-      else
-        v[i] = __uint_as_float(r[c * ACC + i]);
+      if constexpr (SWIGLU) v[i] = mx_swiglu7(__uint_as_float(rc[2 * i]), __uint_as_float(rc[2 * i + 1]));
+      else v[i] = __uint_as_float(rc[i]);
     }
     if (p.row_weights) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) v[i] *= rw;
     }
-    __syncwarp();                                   // the chunk before has left the staging
+    uint32_t w[8];
 #pragma unroll
-    for (int k = 0; k < MG_STG_WIDE / 16; ++k) {
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if constexpr (OUT == DT_F32) w[j] = __float_as_uint(v[4 * k + j]);
-        else w[j] = mg_pack16<OUT>(v[8 * k + 2 * j], v[8 * k + 2 * j + 1]);
-      }
-      *reinterpret_cast<uint4*>(stg + mg_stg<MG_STG_WIDE>(lane, k)) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (OUT == DT_F32) w[j] = __float_as_uint(v[j]);
+      else w[j] = mg_pack16<OUT>(v[2 * j], v[2 * j + 1]);
     }
-    __syncwarp();
-    const int o0 = SWIGLU ? (col0 + c * ACC) / 2 : col0 + c * ACC;
-    mg_store_rows<ESZ, MG_STG_WIDE>(p, stg, t.row0 + m0, min(32, t.rows - m0), o0, n_out - o0, lane);
+    if (p.y_vec32) {
+      if (live && o0 + c * PER < n_out) st_global_32(dst + c * 32, w);
+    } else {
+      __syncwarp();                                 // the chunk before has left the staging
+      *reinterpret_cast<uint4*>(stg + mg_stg<MG_STG_WIDE>(lane, 0)) = make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint4*>(stg + mg_stg<MG_STG_WIDE>(lane, 1)) = make_uint4(w[4], w[5], w[6], w[7]);
+      __syncwarp();
+      mg_store_rows<ESZ, MG_STG_WIDE>(p, stg, t.row0 + m0, min(32, t.rows - m0), o0 + c * PER, n_out - o0 - c * PER,
+                                      lane);
+    }
   }
 }
 
@@ -333,19 +344,20 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     const bool one = elect_one();
     int64_t issued = 0;
     const uint32_t wblk = (uint32_t)((p.N + 127) / 128);
-    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int4 next = mg_fetch(p, t0 < total ? t0 / p.n_wt : 0);
     int trow = 0, wrow = 0;
     const uint8_t *sf_t = nullptr, *sf_w = nullptr;
     bool second = false;                                            // the weight tile's second atom block exists
     mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int t, int kb, int s, uint32_t phase) {
       if (kb == 0) {
         const int wt = t % p.n_wt;
-        trow = (int)next.row0;
-        wrow = next.e * p.N + wt * S::BN;
-        sf_t = p.sf_tok + (uint64_t)next.slot * p.katoms * 512;
-        sf_w = p.sf_w + ((uint64_t)next.e * wblk + wt * 2) * p.katoms * 512;
+        const MgTile tile = mg_tile<S::SLOT>(p, next);
+        trow = (int)tile.row0;
+        wrow = tile.e * p.N + wt * S::BN;
+        sf_t = p.sf_tok + (uint64_t)tile.slot * p.katoms * 512;
+        sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wt * 2) * p.katoms * 512;
         second = wt * 2 + 1 < (int)wblk;
-        if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
+        if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       }
       if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       if (one) {
@@ -410,11 +422,11 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     const int slice = (warp - 2) >> 2;             // accumulator columns [64 * slice, +64)
     uint8_t* stg = sSTG + (warp - 2) * 32 * MG_STG_WIDE;
     uint32_t acc_phase = 0;
-    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int4 next = mg_fetch(p, t0 < total ? t0 / p.n_wt : 0);
     for (int t = t0; t < total; t += step) {
       const int wt = t % p.n_wt;
-      const MgTile tile = next;
-      if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
+      const MgTile tile = mg_tile<S::SLOT>(p, next);
+      if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       if (!mbar_wait(smem_u32(tfull_bar), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
       acc_phase ^= 1;
       tc_fence_after();
@@ -514,17 +526,18 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     const bool one = elect_one();
     int64_t issued = 0;
     const uint32_t wblk = (uint32_t)((p.N + 127) / 128);
-    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int4 next = mg_fetch(p, t0 < total ? t0 / p.n_wt : 0);
     int trow = 0, wrow = 0;
     const uint8_t *sf_t = nullptr, *sf_w = nullptr;
     mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int t, int kb, int s, uint32_t phase) {
       if (kb == kb0) {
         const int wt = t % p.n_wt;
-        trow = (int)next.row0;
-        wrow = next.e * p.N + wt * 128;
-        sf_t = p.sf_tok + (uint64_t)next.slot * p.katoms * 512;
-        sf_w = p.sf_w + ((uint64_t)next.e * wblk + wt) * p.katoms * 512;
-        if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
+        const MgTile tile = mg_tile<S::SLOT>(p, next);
+        trow = (int)tile.row0;
+        wrow = tile.e * p.N + wt * 128;
+        sf_t = p.sf_tok + (uint64_t)tile.slot * p.katoms * 512;
+        sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wt) * p.katoms * 512;
+        if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       }
       if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
       if (one) {
@@ -591,11 +604,11 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     uint8_t* stg = sSTG + (warp - 2) * 32 * MG_STG_FLAT;
     int acc = 0;
     uint32_t acc_phase = 0;
-    MgTile next = t0 < total ? mg_tile<S::SLOT>(p, t0 / p.n_wt) : MgTile{};
+    int4 next = mg_fetch(p, t0 < total ? t0 / p.n_wt : 0);
     for (int t = t0; t < total; t += step) {
       const int wt = t % p.n_wt;
-      const MgTile tile = next;
-      if (t + step < total) next = mg_tile<S::SLOT>(p, (t + step) / p.n_wt);
+      const MgTile tile = mg_tile<S::SLOT>(p, next);
+      if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       const int n0 = wt * 128 + q * 32;
       const float b = p.bias && n0 + lane < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n0 + lane) : 0.f;
       if (!mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
@@ -637,7 +650,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     cluster_sync();
     if (t0 < total) {
       const int tt = t0 / p.n_wt, wt = t0 % p.n_wt;
-      const MgTile tile = mg_tile<S::SLOT>(p, tt);
+      const MgTile tile = mg_tile<S::SLOT>(p, mg_fetch(p, tt));
       const uint32_t red = smem_u32(smem);
       uint32_t peer[8];
 #pragma unroll
@@ -1071,6 +1084,7 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
   a.y_dtype = p.y_dtype;
   a.y_stride = p.y_stride;
   a.y_vec = (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && p.y_stride * y_esz % 16 == 0 && n_out * y_esz % 16 == 0;
+  a.y_vec32 = (reinterpret_cast<uintptr_t>(p.y) & 31) == 0 && p.y_stride * y_esz % 32 == 0 && n_out * y_esz % 32 == 0;
   a.status = p.status;
   a.timeout_ns = p.timeout_ns;
   CUtensorMap tt, tw;
