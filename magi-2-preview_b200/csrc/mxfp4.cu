@@ -43,7 +43,10 @@ __global__ void __launch_bounds__(MXQ_THREADS)
   }
 }
 
-// Sixteen threads take one atom column, 8 columns each (a 16-B store in a 2-byte type).
+// Sixteen threads take one atom column, 8 columns each (a 16-B store in a 2-byte type), and MXD_UN
+// items a grid apart, so that as many loads of 5 B are in flight a thread (268 M elements to bf16:
+// 138 us with one, 4.9 TB/s, 124 with four).
+constexpr int MXD_UN = 4;
 template <int DT>
 __global__ void __launch_bounds__(MXQ_THREADS)
     mx_dequantize_kernel(const uint8_t* __restrict__ data, const uint8_t* __restrict__ sf, FastDiv rows,
@@ -53,26 +56,41 @@ __global__ void __launch_bounds__(MXQ_THREADS)
   pdl_trigger();
   using T = typename MxType<DT>::T;
   const int sub = threadIdx.x & 15;
-  for (uint32_t it = blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it < items;
-       it += gridDim.x * (MXQ_THREADS / 16)) {
-    const uint32_t rr = katoms.div(it), ka = it - rr * katoms.d;
-    const uint32_t b = rows.div(rr), row = rr - b * rows.d;
-    const uint32_t c0 = ka * 128 + sub * 8;
-    if (c0 >= cols) continue;
-    const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(data + (uint64_t)it * 64 + sub * 4));
-    const float s = mx_scale_value(__ldg(sf + (uint64_t)b * (rows_p >> 7) * katoms.d * 512 +
-                                         mx_sf_offset(row, ka * 4 + (sub >> 2), katoms.d)));
-    float v[8];
-    mx_decode8(w, v);
-    T* o = out + (uint64_t)rr * cols + c0;
-    if (vec_ok && c0 + 8 <= cols) {
-      __align__(16) T t[8];
+  const uint32_t hop = gridDim.x * (MXQ_THREADS / 16);
+  for (uint32_t it0 = blockIdx.x * (MXQ_THREADS / 16) + (threadIdx.x >> 4); it0 < items; it0 += hop * MXD_UN) {
+    uint32_t w[MXD_UN], sb[MXD_UN], c0[MXD_UN];
+    T* o[MXD_UN];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mx_store(&t[i], v[i] * s);
+    for (int u = 0; u < MXD_UN; ++u) {
+      const uint32_t it = it0 + u * hop;
+      const uint32_t rr = katoms.div(it), ka = it - rr * katoms.d;
+      const uint32_t b = rows.div(rr), row = rr - b * rows.d;
+      c0[u] = it < items ? ka * 128 + sub * 8 : cols;
+      o[u] = out + (uint64_t)rr * cols + c0[u];
+      w[u] = 0;
+      sb[u] = 0;
+      if (c0[u] < cols) {
+        w[u] = __ldg(reinterpret_cast<const uint32_t*>(data + (uint64_t)it * 64 + sub * 4));
+        sb[u] = __ldg(sf + (uint64_t)b * (rows_p >> 7) * katoms.d * 512 +
+                      mx_sf_offset(row, ka * 4 + (sub >> 2), katoms.d));
+      }
+    }
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(o)[i] = reinterpret_cast<const uint4*>(t)[i];
-    } else {
-      for (uint32_t i = 0; i < min(8u, cols - c0); ++i) mx_store(o + i, v[i] * s);
+    for (int u = 0; u < MXD_UN; ++u) {
+      if (c0[u] >= cols) continue;
+      const float s = mx_scale_value(sb[u]);
+      float v[8];
+      mx_decode8(w[u], v);
+      if (vec_ok && c0[u] + 8 <= cols) {
+        __align__(16) T t[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx_store(&t[i], v[i] * s);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+          reinterpret_cast<uint4*>(o[u])[i] = reinterpret_cast<const uint4*>(t)[i];
+      } else {
+        for (uint32_t i = 0; i < min(8u, cols - c0[u]); ++i) mx_store(o[u] + i, v[i] * s);
+      }
     }
   }
 }
@@ -107,9 +125,9 @@ cudaError_t launch_mx_dequantize(const uint8_t* data, const uint8_t* sf, int64_t
   const int64_t rows_p = (rows + 127) / 128 * 128, katoms = mx_padded_cols(cols) / 128;
   const int64_t items = n * rows * katoms;
   if (items == 0) return cudaSuccess;
-  if (items >= (int64_t)1 << 31) return cudaErrorInvalidValue;
+  if (items >= (int64_t)1 << 30) return cudaErrorInvalidValue;      // above 2^37 elements (an item number stays below 2^31)
   const bool vec = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && cols * (dtype == DT_F32 ? 4 : 2) % 16 == 0;
-  const unsigned grid = mx_grid(items, MXQ_THREADS / 16);
+  const unsigned grid = mx_grid(items, MXQ_THREADS / 16 * MXD_UN);
 #define MX_D(DT)                                                                                                 \
   MHMOE_LAUNCH_PDL(mx_dequantize_kernel<DT>, grid, MXQ_THREADS, 0, st, data, sf, FastDiv((uint32_t)rows),        \
                    (uint32_t)rows_p, (uint32_t)cols, FastDiv((uint32_t)katoms), (uint32_t)items, vec,            \
