@@ -251,7 +251,7 @@ MHMOE_API int mhmoe_mxfp4_dequantize(const uint8_t* data, const uint8_t* scales,
                                      int out_dtype, void* out, void* stream);
 
 /* Scratch bytes of the two products below: x_rows activation rows, R output rows, n weight
- * matrices [N, cols] (n = 1 and R = x_rows for mhmoe_mxfp4_linear). */
+ * matrices [N, cols] (n = 1 and R = x_rows for mhmoe_mxfp4_linear); 0 where none is needed. */
 MHMOE_API size_t mhmoe_mxfp4_workspace_bytes(int64_t x_rows, int64_t R, int n_experts, int N, int cols, int grouped);
 
 /* y [M, N'] = act(Q(x) W^T + bias) with W an MXFP4 matrix [N, cols], sums in fp32, one rounding to

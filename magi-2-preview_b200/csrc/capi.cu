@@ -376,8 +376,8 @@ int mhmoe_mxfp4_linear(const void* x, int x_dtype, int64_t x_stride, const uint8
   MHMOE_REQUIRE(w_data && w_scales && aligned16(w_data) && aligned16(w_scales));
   if (M > 0) {
     MHMOE_REQUIRE(y && y_stride >= (activation ? N / 2 : N));
-    MHMOE_REQUIRE((x && workspace && aligned16(workspace)) ||
-                  (!x && x_data && x_scales && aligned16(x_data) && aligned16(x_scales)));
+    MHMOE_REQUIRE(x || (x_data && x_scales && aligned16(x_data) && aligned16(x_scales)));
+    if (x && mx_product_workspace_bytes(M, M, 1, N, cols, false) > 0) MHMOE_REQUIRE(workspace && aligned16(workspace));
   }
   MHMOE_CHECK_ARCH();
   if (M == 0) return MHMOE_OK;

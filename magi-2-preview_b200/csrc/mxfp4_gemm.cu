@@ -59,6 +59,10 @@ struct FlatShape {
 };
 
 struct MgParams {
+  const void* x;              // rows that the flat kernel quantises itself
+  int64_t x_stride;
+  int cols;
+  bool ceil, x_vec;
   const uint8_t* sf_tok;      // scale atoms of the token tiles, a 128-row block per slot
   const uint8_t* sf_w;
   const int4* tiles;          // grouped: {expert, first row, rows, slot}; null: dense
@@ -459,7 +463,11 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
 // Flat kernel.  tmT: token rows [R, cols_p/2], box 128 B x BN; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 128.  SPLIT: a cluster of CTAs shares one work item along the columns; their partial
 // accumulators meet in distributed shared memory and are summed in the order of the ranks.
-template <int BN, bool SPLIT, int OUT>
+//
+// XQ (with SPLIT, where a CTA has one item): the type of the up to BN rows of x that the epilogue warps
+// quantise into operand B's stages themselves, before they have outputs to write, instead of a
+// kernel ahead of this one (one token x 4096 x 2048: 8.1 us, 11.3 with the two kernels).
+template <int BN, bool SPLIT, int OUT, int XQ>
 __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     mx_flat_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
                    const __grid_constant__ MgParams p) {
@@ -481,13 +489,14 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   uint64_t* drain_bar = tempty_bar + NACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   static_assert((2 * STAGES + 2 * NACC + 1) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  static_assert(XQ < 0 || (SPLIT && BN <= 32 && EPW == 4), "a stage of rows is quantised by 128 threads");
   static_assert(!SPLIT || BN * 128 * 4 <= STAGES * MG_A_BYTES, "partial sums lie over operand A's stages");
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
   const int lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&full_bar[s]), XQ >= 0 ? 1 + EPW : 1);
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int a = 0; a < NACC; ++a) {
@@ -496,7 +505,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     }
     mbar_init(smem_u32(drain_bar), 1);
     fence_mbar_init();
-    tma_prefetch_desc(&tmT);
+    if (XQ < 0) tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
   }
   if (warp == 1) {
@@ -543,11 +552,13 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       if (one) {
         const uint32_t fb = smem_u32(&full_bar[s]);
         const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;      // atoms of this stage
-        mbar_arrive_expect_tx(fb, MG_A_BYTES + S::B_BYTES + sfn * 2);
+        mbar_arrive_expect_tx(fb, MG_A_BYTES + sfn + (XQ < 0 ? S::B_BYTES + sfn : 0));
         tma_load_2d(smem_u32(sA + s * MG_A_BYTES), &tmW, fb, kb * (MG_BK / 2), wrow);
-        tma_load_2d(smem_u32(sB + s * S::B_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
         bulk_load(smem_u32(sSFA + s * MG_SF_BYTES), sf_w + kb * 1024, sfn, fb);
-        bulk_load(smem_u32(sSFB + s * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
+        if constexpr (XQ < 0) {
+          tma_load_2d(smem_u32(sB + s * S::B_BYTES), &tmT, fb, kb * (MG_BK / 2), trow);
+          bulk_load(smem_u32(sSFB + s * MG_SF_BYTES), sf_t + kb * 1024, sfn, fb);
+        }
       }
       __syncwarp();
       ++issued;
@@ -602,6 +613,36 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     const int part = (warp - 2) >> 2;          // with 8 warps: every other chunk of columns
     constexpr int NC = BN < 32 ? BN : 32;
     uint8_t* stg = sSTG + (warp - 2) * 32 * MG_STG_FLAT;
+    if constexpr (XQ >= 0) {
+      // 16 threads a row, 16 columns each; rows behind the last hold what was there: their columns of
+      // the accumulator are not stored
+      using T = typename MxType<XQ < 0 ? 0 : XQ>::T;
+      const int tid = threadIdx.x - 64, chunk = tid & 15;
+      const uint32_t mask = 0xffu << (lane & 24);
+      mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
+        if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+        const int c0 = kb * MG_BK + chunk * 16;
+#pragma unroll
+        for (int row = tid >> 4; row < BN; row += 8) {
+          if (row >= (int)p.R) break;              // the same for the 16 threads of a row
+          MxRaw16<T> v;
+          const bool live = c0 < p.cols;
+          v.load(static_cast<const T*>(p.x) + row * p.x_stride + c0, live && p.x_vec && c0 + 16 <= p.cols,
+                 live ? min(16, p.cols - c0) : 0);
+          uint2 code;
+          const uint32_t sw = mx_quantize16(v, p.ceil, chunk & 7, mask, code);
+          // 128-B swizzle: 16-B chunk k of row r sits at chunk k ^ (r & 7)
+          *reinterpret_cast<uint2*>(sB + s * S::B_BYTES + row * 128 + (((chunk >> 1) ^ (row & 7)) << 4) +
+                                    (chunk & 1) * 8) = code;
+          if ((chunk & 7) == 0)
+            *reinterpret_cast<uint32_t*>(sSFB + s * MG_SF_BYTES + (chunk >> 3) * 512 + row * 16) = sw;
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&full_bar[s]));
+        return true;
+      });
+    }
     int acc = 0;
     uint32_t acc_phase = 0;
     int4 next = mg_fetch(p, t0 < total ? t0 / p.n_wt : 0);
@@ -891,6 +932,7 @@ struct MgPlan {
   int64_t tiles, slots;       // token tiles at most; scale slots
   int n_wt;
   bool once;                  // quantise the tokens first, then copy their rows
+  bool own;                   // the flat kernel quantises x itself
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -921,6 +963,7 @@ MgPlan mg_plan(int64_t x_rows, int64_t R, int n, int N, int64_t katoms, bool gro
   // Copying a row costs a third of quantising it, a launch more about 2 us (top-8 of 128 experts, 1024
   // columns: 8192 rows 16.1 us quantised each, 17.7 copied; 32768 rows 38.3 and 30.8).
   g.once = grouped && R >= 2 * x_rows && R >= 16384;
+  g.own = !grouped && R <= 16 && g.n_wt <= sms;     // one item a CTA
   g.split = 1;
   const int64_t n_kblk = ceil_div(katoms, 2);
   while (g.flat && g.split < 8 && g.tiles * g.n_wt * g.split * 2 <= sms && g.split * 2 <= n_kblk) g.split *= 2;
@@ -956,11 +999,11 @@ cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
                     tt, tw, p);
 }
 
-template <int BN, bool SPLIT, int OUT>
+template <int BN, bool SPLIT, int OUT, int XQ = -1>
 cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
                         cudaStream_t st) {
   using S = FlatShape<BN>;
-  auto kernel = mx_flat_kernel<BN, SPLIT, OUT>;
+  auto kernel = mx_flat_kernel<BN, SPLIT, OUT, XQ>;
   static PerDeviceOnce once;
   const cudaError_t attr = once.run(
       [&](int) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM); });
@@ -991,10 +1034,10 @@ cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
 template <int BN>
 cudaError_t launch_flat(const CUtensorMap& tt, const CUtensorMap& tw, const MgParams& p, const MgPlan& g,
                         cudaStream_t st) {
-  if (g.split > 1) return launch_flat<BN, true, DT_F32>(tt, tw, p, g, st);      // stores by p.y_dtype
-  return p.y_dtype == DT_F32    ? launch_flat<BN, false, DT_F32>(tt, tw, p, g, st)
-         : p.y_dtype == DT_BF16 ? launch_flat<BN, false, DT_BF16>(tt, tw, p, g, st)
-                                : launch_flat<BN, false, DT_F16>(tt, tw, p, g, st);
+  if (g.split > 1) return launch_flat<BN, true, DT_F32, -1>(tt, tw, p, g, st);      // stores by p.y_dtype
+  return p.y_dtype == DT_F32    ? launch_flat<BN, false, DT_F32, -1>(tt, tw, p, g, st)
+         : p.y_dtype == DT_BF16 ? launch_flat<BN, false, DT_BF16, -1>(tt, tw, p, g, st)
+                                : launch_flat<BN, false, DT_F16, -1>(tt, tw, p, g, st);
 }
 
 template <int OUT>
@@ -1008,7 +1051,8 @@ cudaError_t launch_wide(const CUtensorMap& tt, const CUtensorMap& tw, const MgPa
 size_t mx_product_workspace_bytes(int64_t x_rows, int64_t R, int n, int N, int cols, bool grouped) {
   const int64_t katoms = mx_padded_cols(cols) / 128;
   if (R == 0) return 0;
-  return mg_scratch(mg_plan(x_rows, R, n, N, katoms, grouped), x_rows, R, katoms, grouped).bytes;
+  const MgPlan g = mg_plan(x_rows, R, n, N, katoms, grouped);
+  return g.own ? 0 : mg_scratch(g, x_rows, R, katoms, grouped).bytes;
 }
 
 int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t* cerr) {
@@ -1016,6 +1060,7 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
   const bool grouped = p.offsets != nullptr;
   const MgPlan g = mg_plan(p.x_rows, p.R, p.n, p.N, katoms, grouped);
   if (g.tiles * g.n_wt >= (int64_t)1 << 30) return MHMOE_ERR_CAPACITY;
+  const bool own = g.own && !p.xq;
   const MgScratch ws = mg_scratch(g, p.x_rows, p.R, katoms, grouped);
   uint8_t* base = static_cast<uint8_t*>(workspace);
   const int64_t y_esz = p.y_dtype == DT_F32 ? 4 : 2, n_out = p.act ? p.N / 2 : p.N;
@@ -1065,7 +1110,7 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
     a.sf_tok = q.sf;
     a.tiles = q.tiles;
     a.n_tiles = q.n_tiles;
-  } else if (!p.xq) {
+  } else if (!p.xq && !own) {
     *cerr = launch_mx_quantize(p.x, p.x_dtype, 0, p.x_stride, 1, p.R, p.cols, p.ceil, base + ws.data, base + ws.sf, st);
     data = base + ws.data;
     a.sf_tok = base + ws.sf;
@@ -1087,11 +1132,21 @@ int mx_product(const MxProduct& p, void* workspace, cudaStream_t st, cudaError_t
   a.y_vec32 = (reinterpret_cast<uintptr_t>(p.y) & 31) == 0 && p.y_stride * y_esz % 32 == 0 && n_out * y_esz % 32 == 0;
   a.status = p.status;
   a.timeout_ns = p.timeout_ns;
-  CUtensorMap tt, tw;
-  if (encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)g.slot_rows) != cudaSuccess ||
+  CUtensorMap tt{}, tw;
+  if ((!own && encode_tmap_2d_u8(&tt, data, (uint64_t)katoms * 64, (uint64_t)p.R, 128, (uint32_t)g.slot_rows) !=
+                   cudaSuccess) ||
       encode_tmap_2d_u8(&tw, p.w_data, (uint64_t)katoms * 64, (uint64_t)p.n * p.N, 128, g.flat ? 128 : 256) != cudaSuccess)
     return MHMOE_ERR_DRIVER;
-  if (g.flat)
+  if (own) {
+    a.x = p.x;
+    a.x_stride = p.x_stride;
+    a.cols = p.cols;
+    a.ceil = p.ceil;
+    a.x_vec = (reinterpret_cast<uintptr_t>(p.x) & 15) == 0 && p.x_stride * (p.x_dtype == DT_F32 ? 4 : 2) % 16 == 0;
+    *cerr = p.x_dtype == DT_F32    ? launch_flat<16, true, DT_F32, DT_F32>(tt, tw, a, g, st)
+            : p.x_dtype == DT_BF16 ? launch_flat<16, true, DT_F32, DT_BF16>(tt, tw, a, g, st)
+                                   : launch_flat<16, true, DT_F32, DT_F16>(tt, tw, a, g, st);
+  } else if (g.flat)
     *cerr = g.bn == 16   ? launch_flat<16>(tt, tw, a, g, st)
             : g.bn == 32 ? launch_flat<32>(tt, tw, a, g, st)
             : g.bn == 64 ? launch_flat<64>(tt, tw, a, g, st)

@@ -94,7 +94,7 @@ class MXFP4Matrix:
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(x_rows: int, R: int, n: int, N: int, cols: int, grouped: int, device: int) -> int:
     with torch.cuda.device(device):
-        return max(1, _lib.lib().mhmoe_mxfp4_workspace_bytes(x_rows, R, n, N, cols, grouped))
+        return _lib.lib().mhmoe_mxfp4_workspace_bytes(x_rows, R, n, N, cols, grouped)
 
 
 def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -218,7 +218,9 @@ def mxfp4_linear(x: torch.Tensor | MXFP4Matrix, weight: MXFP4Matrix, bias: torch
         if cols > 1 and x2.stride(1) != 1:
             x2 = x2.detach().contiguous()
         xd, xs = _lib.DTYPES[x.dtype], x2.stride(0)
-        ws = torch.empty(_workspace_bytes(M, M, 1, N, cols, 0, dev.index), dtype=torch.uint8, device=dev)
+        nbytes = _workspace_bytes(M, M, 1, N, cols, 0, dev.index)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _lib.launch("mhmoe_mxfp4_linear", dev, _lib.ptr(x2), xd, xs, xq, xsf, M, cols, rounding, weight.data.data_ptr(),
                 weight.sf.data_ptr(), N, _lib.ptr(bias), act, _lib.ptr(ws), y.data_ptr(), _lib.DTYPES[dtype], n_out,
                 _lib.device_status(dev).data_ptr(), 0)
@@ -235,8 +237,8 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
         y[r] = row_weights[r] * act(Q(x[gather_ids[r]]) W_e^T + bias_e),
         expert_offsets[e] <= r < expert_offsets[e + 1]
 
-    x [T, cols] (fp32, bf16 or fp16); weight [n, N, cols]; expert_offsets int64 [n + 1] on the
-    device; gather_ids int32 [R] (default: row r of x itself, R = T); row_weights [R]; bias [n, N];
+    x [T, cols] (fp32, bf16 or fp16); weight [n, N, cols]; expert_offsets int64 (or
+    int32) [n + 1] on the device; gather_ids int32 [R] (default: row r of x itself, R = T); row_weights [R]; bias [n, N];
     activation, out_dtype and scale_rounding as in ``mxfp4_linear``.
 
     Returns y [R, N] (N/2 with SwiGLU7).  The rows from ``expert_offsets[n]`` on belong to no
@@ -256,8 +258,10 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
         raise ValueError(f"weight {weight.shape} is not [n, N, {cols}]")
     if tuple(expert_offsets.shape) != (n + 1,):
         raise ValueError(f"expert_offsets must be [{n + 1}], got {tuple(expert_offsets.shape)}")
-    if gather_ids is not None and (gather_ids.dim() != 1 or gather_ids.is_floating_point()):
-        raise ValueError("gather_ids must be a vector of row numbers")
+    if expert_offsets.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"expert_offsets must be int64 or int32, got {expert_offsets.dtype}")
+    if gather_ids is not None and (gather_ids.dim() != 1 or gather_ids.dtype != torch.int32):
+        raise ValueError(f"gather_ids must be an int32 vector, got {tuple(gather_ids.shape)} {gather_ids.dtype}")
     R = T if gather_ids is None else gather_ids.numel()
     if row_weights is not None and tuple(row_weights.shape) != (R,):
         raise ValueError(f"row_weights must be [{R}], got {tuple(row_weights.shape)}")
@@ -273,10 +277,10 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
     if cols > 1 and x.stride(1) != 1:
         x = x.detach().contiguous()
     offs = _as(expert_offsets, torch.int64)
-    gids = None if gather_ids is None else _as(gather_ids, torch.int32)
+    gids = gather_ids if gather_ids is None or gather_ids.is_contiguous() else gather_ids.contiguous()
     rw = None if row_weights is None else _as(row_weights, torch.float32)
     y = torch.empty((R, n_out), dtype=dtype, device=dev) if out is None else out
-    ws = torch.empty(_workspace_bytes(T, R, n, N, cols, 1, dev.index), dtype=torch.uint8, device=dev)
+    ws = torch.empty(max(1, _workspace_bytes(T, R, n, N, cols, 1, dev.index)), dtype=torch.uint8, device=dev)
     _lib.launch("mhmoe_mxfp4_expert_linear", dev, x.data_ptr(), _lib.DTYPES[x.dtype], x.stride(0), T, cols, rounding,
                 weight.data.data_ptr(), weight.sf.data_ptr(), n, N, offs.data_ptr(), _lib.ptr(gids), R, _lib.ptr(rw),
                 _lib.ptr(bias), act, ws.data_ptr(), y.data_ptr(), _lib.DTYPES[dtype], max(y.stride(0), n_out),

@@ -107,7 +107,7 @@ def _linear(L, x=P, xd=0, xq=None, M=4, cols=64, rounding=0, w=P, N=32, act=0, w
 
 
 @pytest.mark.parametrize("bad", [dict(x=None), dict(xd=4), dict(M=-1), dict(cols=0), dict(rounding=2), dict(w=None),
-                                 dict(w=P + 8), dict(N=0), dict(act=2), dict(act=1, N=31), dict(ws=None), dict(ws=P + 4),
+                                 dict(w=P + 8), dict(N=0), dict(act=2), dict(act=1, N=31), dict(M=200, ws=None), dict(M=200, ws=P + 4),
                                  dict(y=None), dict(yd=-1), dict(ys=31), dict(cols=(1 << 20) + 1)])
 def test_linear_refuses(L, bad):
     assert _linear(L, **bad) == ERR_ARGS
@@ -117,6 +117,10 @@ def test_linear_accepts(L):
     assert _linear(L) == ERR_ARCH
     assert _linear(L, x=None, xq=P, ws=None) == ERR_ARCH
     assert _linear(L, act=1, ys=16) == ERR_ARCH
+    # a few rows need no workspace
+    assert L.mhmoe_mxfp4_workspace_bytes(4, 4, 1, 32, 64, 0) == 0
+    assert _linear(L, ws=None) == ERR_ARCH
+    assert L.mhmoe_mxfp4_workspace_bytes(200, 200, 1, 32, 64, 0) > 0
 
 
 def _experts(L, x=P, x_rows=8, cols=64, n=4, N=32, offs=P, gids=None, R=8, ws=P, ys=32):
