@@ -35,6 +35,7 @@ import torch.nn.functional as F
 from . import _lib
 from .fwd import ffn_nvfp4
 from .moe import CoreMultiHeadMoE, CoreMultiHeadMoEConfig, _same_key
+from .mxfp4 import MXFP4Matrix, mxfp4_linear, mxfp4_quantize
 from .nvfp4 import pack_down, pack_gate_up
 
 
@@ -57,6 +58,8 @@ class MoEConfig:
     modality_specific_expert_intermediate_size: int = 1280
     num_heads: int = 12
     split_merge_intermediate_size: Optional[int] = None
+    num_expert_groups: int = 1        # see CoreMultiHeadMoEConfig
+    topk_expert_groups: int = 1
 
 
 @dataclass
@@ -72,6 +75,9 @@ class MultiHeadMoELayerConfig:
     shared_expert_params_dtype: torch.dtype
     split_merge_intermediate_size: Optional[int]
     moe_config: MoEConfig
+    # "bf16": the split and merge linears are library GEMMs; "mxfp4": their weights are held in MXFP4
+    # and the activations quantised on the way (flash_mh_moe.mxfp4; no reference key)
+    linear_format: str = "bf16"
 
 
 def group_layout(modality_dispatcher, rows: int, num_modality: int,
@@ -179,6 +185,8 @@ class MultiHeadMoELayer(nn.Module):
         act = config.activation_type
         if (act.value if isinstance(act, Enum) else str(act)) != MLPActivationType.SWIGLU7.value:
             raise ValueError(f"Unknown activation type: {act}")
+        if config.linear_format not in ("bf16", "mxfp4"):
+            raise ValueError(f"Unknown linear format: {config.linear_format}")
         self.config = config
         mc = config.moe_config
         moe_hidden = config.split_merge_intermediate_size or config.hidden_size
@@ -186,7 +194,8 @@ class MultiHeadMoELayer(nn.Module):
             hidden_size=moe_hidden, num_heads=mc.num_heads, num_experts=mc.num_experts, top_k=mc.top_k,
             expert_intermediate_size=mc.expert_intermediate_size, num_layers=config.num_layers,
             params_dtype=config.params_dtype, score_func=mc.score_func, route_norm=mc.route_norm,
-            route_scale=mc.route_scale), ep_group=ep_group)
+            route_scale=mc.route_scale, num_expert_groups=mc.num_expert_groups,
+            topk_expert_groups=mc.topk_expert_groups), ep_group=ep_group)
         self.is_swiglu = True
         d, M = config.hidden_size, config.num_modality
         Is, Im = config.shared_expert_intermediate_sizes, config.modality_specific_expert_intermediate_sizes
@@ -203,6 +212,7 @@ class MultiHeadMoELayer(nn.Module):
         self._shared_packed = None
         self._shared_key = None
         self._routing_cache: dict = {}
+        self._linear_packed: dict = {}
 
     # ── shared experts as an NVFP4 expert set: expert 0 = shared, expert 1 + m = modality m ──
     def _shared_params(self):
@@ -265,14 +275,30 @@ class MultiHeadMoELayer(nn.Module):
                       deterministic=True)
         return y.view(S, d)
 
+    def _linear_mxfp4(self, name: str) -> MXFP4Matrix:
+        """The MXFP4 form of ``split_linear`` / ``merge_linear``, packed again when its parameter changes."""
+        w = getattr(self, name).weight
+        key = ((w, w.data_ptr(), w._version),)
+        hit = self._linear_packed.get(name)
+        if hit is None or not _same_key(hit[0], key):
+            hit = (key, mxfp4_quantize(w))
+            self._linear_packed[name] = hit
+        return hit[1]
+
     def forward(self, hidden_states: torch.Tensor, modality_dispatcher=None) -> torch.Tensor:
         _lib.require_cuda(hidden_states)
         shape = hidden_states.shape
         x = hidden_states.reshape(-1, self.config.hidden_size)
         sizes, cu = group_layout(modality_dispatcher, x.shape[0], self.config.num_modality, x.device)
         norm_output = self.pre_norm(x, cu_groups=cu)
-        moe_out = self.moe_mlp(F.linear(norm_output, self.split_linear.weight))
+        mx = self.config.linear_format == "mxfp4"
+        split = (mxfp4_linear(norm_output, self._linear_mxfp4("split_linear")) if mx
+                 else F.linear(norm_output, self.split_linear.weight))
+        moe_out = self.moe_mlp(split)
         shared = self._shared_expert_forward(norm_output, sizes)
+        if mx:                                    # added in fp32, rounded once
+            merged = mxfp4_linear(moe_out, self._linear_mxfp4("merge_linear"), out_dtype=torch.float32)
+            return merged.add_(shared).to(shared.dtype).view(shape)
         # merge_linear(moe_out) + shared in one GEMM (accumulating onto the shared output)
         out = torch.addmm(shared, moe_out, self.merge_linear.weight.t())
         return out.view(shape)

@@ -28,7 +28,7 @@ import torch.nn as nn
 from .fwd import ffn_nvfp4
 from .nvfp4 import NVFP4Down, NVFP4GateUp, pack_down, pack_gate_up
 from .route import (compute_topk_probs_and_indices, flash_mh_moe_global_sort_with_inverse,
-                    fused_router_supported, route_fused, router_logits, router_prepare)
+                    fused_router_supported, route_experts, route_fused, router_logits, router_prepare)
 
 
 def _same_key(a, b) -> bool:
@@ -51,6 +51,10 @@ class CoreMultiHeadMoEConfig:
     route_norm: bool = True
     route_scale: float = 1.0
     recompute_once_in_bwd: bool = True
+    # expert groups of the router (no reference key): only the experts of the topk_expert_groups best
+    # of num_expert_groups equal groups are candidates (flash_mh_moe.route.route_experts)
+    num_expert_groups: int = 1
+    topk_expert_groups: int = 1
 
 
 # Modules by their op key.  Weak values: registering a module does not keep it (and its
@@ -187,6 +191,12 @@ class CoreMultiHeadMoE(nn.Module):
     def _route(self, x_heads: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """magi2_preview.py:2588-2601: fp32 logits -> top-k -> x route_scale."""
         bias = self.router.expert_bias.view(self.num_heads, self.num_experts)
+        if self.config.num_expert_groups > 1:
+            return route_experts(
+                router_logits(x_heads, self.gate, self.num_experts), self.topk, score_func=self.config.score_func,
+                expert_bias=bias, num_groups=self.config.num_expert_groups,
+                topk_groups=self.config.topk_expert_groups, route_norm=self.config.route_norm,
+                route_scale=float(self.config.route_scale))
         if fused_router_supported(self.num_experts, self.topk, self.d_head):
             planes, nsplit = self.router_planes()
             return route_fused(x_heads, planes, nsplit, self.num_experts, self.topk,
