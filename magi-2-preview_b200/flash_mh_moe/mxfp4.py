@@ -50,6 +50,22 @@ class MXFP4Matrix:
     num_matrices: int
     batched: bool
 
+    def __post_init__(self):
+        # the kernels read these sizes: a matrix that does not hold them is refused here
+        n, rows, ka = self.num_matrices, self.rows, _atoms(self.cols)
+        for name, t, size in (("data", self.data, n * rows * ka * 64),
+                              ("sf", self.sf, n * ((rows + 127) // 128) * ka * 512)):
+            if t.dtype != torch.uint8 or t.numel() != size or not t.is_contiguous():
+                raise ValueError(f"MXFP4Matrix.{name} must be {size} contiguous uint8 values for {n} x [{rows}, "
+                                 f"{self.cols}], got {tuple(t.shape)} {t.dtype}")
+        if self.data.device != self.sf.device or n < 0 or rows < 0 or self.cols < 1 or (n != 1 and not self.batched):
+            raise ValueError(f"bad MXFP4Matrix: {n} x [{rows}, {self.cols}], batched {self.batched}, on "
+                             f"{self.data.device} and {self.sf.device}")
+
+    def to(self, device) -> "MXFP4Matrix":
+        return MXFP4Matrix(self.data.to(device), self.sf.to(device), self.rows, self.cols, self.num_matrices,
+                           self.batched)
+
     @property
     def shape(self) -> tuple[int, ...]:
         return (self.num_matrices, self.rows, self.cols) if self.batched else (self.rows, self.cols)
@@ -101,6 +117,13 @@ def _as(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     return t if t.dtype == dtype and t.is_contiguous() else t.detach().to(dtype).contiguous()
 
 
+def _quantized_matrix(data, sf, rows, cols, n, batched) -> MXFP4Matrix:
+    """An MXFP4Matrix of tensors made here, without the constructor's checks."""
+    m = object.__new__(MXFP4Matrix)
+    m.data, m.sf, m.rows, m.cols, m.num_matrices, m.batched = data, sf, rows, cols, n, batched
+    return m
+
+
 def _check_rounding(scale_rounding: str) -> int:
     if scale_rounding not in _ROUNDING:
         raise ValueError(f"scale_rounding must be 'floor' or 'ceil', got {scale_rounding!r}")
@@ -144,7 +167,7 @@ def mxfp4_quantize(x: torch.Tensor, scale_rounding: str = "floor") -> MXFP4Matri
     sf = torch.empty((n, (rows + 127) // 128 * ka * 512), dtype=torch.uint8, device=dev)
     _lib.launch("mhmoe_mxfp4_quantize", dev, x.data_ptr(), _lib.DTYPES[x.dtype], sn, x.stride(-2), n, rows, cols, rounding,
                 data.data_ptr(), sf.data_ptr())
-    return MXFP4Matrix(data, sf, rows, cols, n, batched)
+    return _quantized_matrix(data, sf, rows, cols, n, batched)
 
 
 def mxfp4_dequantize(m: MXFP4Matrix, dtype: torch.dtype = torch.float32) -> torch.Tensor:

@@ -106,6 +106,32 @@ def test_linear_matches(M, N, K, dtype):
     _close(mxfp4_linear(x.cuda(), w, scale_rounding="ceil"), *mx.product(xv, wv[0]))
 
 
+# (rows, weight rows, columns) whose tiles of 128 x 256 are enough for every SM: outputs whose rows start on
+# 32 bytes, on 16, and on neither
+WIDE = [(1300, 4096, 160), (1290, 4104, 130), (1281, 4097, 33), (2500, 2560, 544)]
+
+
+@pytest.mark.parametrize("M,N,K", WIDE)
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_linear_of_many_tiles(M, N, K, dtype):
+    from flash_mh_moe.mxfp4 import mxfp4_linear, mxfp4_quantize
+    x = _x((M, K), dtype, M, spread=False)
+    x[5, :] = float("nan")
+    w, wv = _w(1, N, K, K)
+    w.batched = False
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(1))
+    keep = [r for r in range(0, M, 7) if r != 5] + [M - 1, 127, 128]
+    xv = mx.values(*mx.quantize(x[keep].double().numpy(), "floor"))
+    for kw in (dict(), dict(bias=bias.cuda(), out_dtype=torch.float32), dict(bias=bias.cuda(), activation="swiglu7")):
+        if "activation" in kw and N % 2:
+            continue
+        y = mxfp4_linear(x.cuda(), w, **kw)
+        assert torch.isnan(y[5]).all()
+        _close(y[keep], *mx.product(xv, wv[0], bias.double().numpy() if kw else None, kw.get("activation")))
+        assert torch.equal(torch.nan_to_num(mxfp4_linear(mxfp4_quantize(x.cuda()), w, out_dtype=y.dtype, **{
+            k: v for k, v in kw.items() if k != "out_dtype"})), torch.nan_to_num(y))
+
+
 def test_linear_shapes_strides_and_nan():
     from flash_mh_moe.mxfp4 import mxfp4_linear
     w, wv = _w(1, 96, 160, 0)
@@ -192,6 +218,38 @@ def test_expert_linear_matches(T, E, k, N, K, skew, drop, act, dtype):
     assert (out[used:] == 7).all() and (out[:, 0] == 7).all() and (out[:, -2:] == 7).all()
 
 
+@pytest.mark.parametrize("T,E,k,N,K,skew,drop", [
+    (400, 60, 6, 1030, 96, 0, 0), (700, 100, 4, 512, 160, 2.4, 0.1), (2100, 16, 8, 2560, 64, 1.0, 0.05),
+    (3000, 8, 7, 128, 130, 0, 0)])
+@pytest.mark.parametrize("act", [None, "swiglu7"])
+def test_expert_linear_of_many_rows(T, E, k, N, K, skew, drop, act):
+    """Wide tiles, and (from 16384 rows on) tokens quantised once and copied."""
+    from flash_mh_moe.mxfp4 import mxfp4_expert_linear
+    x = _x((T, K), "bf16", T, spread=False)
+    w, wv = _w(E, N, K, N)
+    gids, rw, offs = _routed(T, E, k, 3, skew, drop)
+    used, o = int(offs[-1]), offs.tolist()
+    bias = 0.5 * torch.randn(E, N, generator=torch.Generator().manual_seed(2))
+    y = mxfp4_expert_linear(x.cuda(), w, offs, gids, rw, bias.cuda(), act)
+    assert (y[used:] == 0).all()
+    xv = mx.values(*mx.quantize(x.double().numpy(), "floor"))
+    g, rwn = gids.cpu().numpy(), rw.cpu().double().numpy()
+    for e in range(E):                                 # every expert's first and last rows and a few between
+        rows = sorted(set(range(o[e], o[e + 1], 37)) | set(range(max(o[e], o[e + 1] - 2), o[e + 1])))
+        if rows:
+            ref, err = mx.product(xv[g[rows]], wv[e], bias[e].double().numpy(), act, rwn[rows])
+            _close(y[rows], ref, err)
+    # ids outside x read as zeros and are reported, copied rows too
+    from flash_mh_moe import _lib
+    _lib.check_device_status(y.device)
+    ids = gids.clone()
+    ids[used // 2] = T
+    z = mxfp4_expert_linear(x.cuda(), w, offs, ids, rw, None, act)
+    with pytest.raises(ValueError):
+        _lib.check_device_status(y.device)
+    assert (z[used // 2] == 0).all()
+
+
 def test_expert_linear_no_rows_and_bad_inputs():
     from flash_mh_moe import _lib
     from flash_mh_moe.mxfp4 import mxfp4_expert_linear
@@ -222,6 +280,8 @@ def test_expert_linear_no_rows_and_bad_inputs():
                  lambda: mxfp4_expert_linear(x, w, offs, out=torch.zeros(10, 64, device="cuda")[:, ::2]),
                  lambda: mxfp4_expert_linear(x, w, offs, out=torch.zeros(9, 64, dtype=torch.bfloat16, device="cuda")),
                  lambda: mxfp4_expert_linear(x.clone().requires_grad_(True), w, offs),
+                 lambda: mxfp4_expert_linear(x, w, offs, gather_ids=ids.long()),
+                 lambda: mxfp4_expert_linear(x, w, offs.float()),
                  lambda: mxfp4_expert_linear(x, w, offs, activation="gelu")]:
         with pytest.raises(ValueError):
             call()

@@ -52,6 +52,18 @@ def test_from_blocks_refuses():
             MXFP4Matrix.from_blocks(*bad)
 
 
+def test_matrix_refuses_sizes_it_does_not_hold():
+    from flash_mh_moe.mxfp4 import MXFP4Matrix
+    d, s = torch.zeros(1, 5, 64, dtype=torch.uint8), torch.zeros(1, 512, dtype=torch.uint8)
+    m = MXFP4Matrix(d, s, 5, 100, 1, False)
+    assert m.to("cpu").shape == (5, 100)
+    for bad in [(d, s, 6, 100, 1, False), (d, s, 5, 129, 1, False), (d, s[:, :100], 5, 100, 1, False),
+                (d.float(), s, 5, 100, 1, False), (d, s, 5, 100, 2, True), (d.transpose(1, 2), s, 5, 100, 1, False),
+                (torch.zeros(2, 5, 64, dtype=torch.uint8), torch.zeros(2, 512, dtype=torch.uint8), 5, 100, 2, False)]:
+        with pytest.raises(ValueError):
+            MXFP4Matrix(*bad)
+
+
 def test_python_refusals_without_a_device():
     from flash_mh_moe import mxfp4
     from flash_mh_moe.route import route_experts
