@@ -6,6 +6,8 @@
 // definition's for every input type.
 //
 // Both kernels are bound by HBM: 2 or 4 bytes an element one way, 17/32 of a byte the other.
+// 268 M elements (n = 16): fp32 quantised in 170 us (7.1 TB/s, codes partly still in L2), to bf16 in
+// 124 us (5.5 TB/s).  A few tokens are bound by the launch: 3.3 and 3.5 us.
 #include "mxfp4.cuh"
 
 namespace mhmoe {
@@ -13,7 +15,7 @@ namespace mhmoe {
 constexpr int MXQ_THREADS = 256;
 
 // Eight threads take one atom column (128 columns of a row), 16 columns each: 8 B of codes a
-// thread, one 4-B word of scales.  Items are (matrix, row, atom column) with the rows of each
+// thread, one 4-B word of scales from four shuffled bytes (a scale needs two threads' maxima).  Items are (matrix, row, atom column) with the rows of each
 // matrix counted to a multiple of 128, so that every scale byte is written.
 template <int DT>
 __global__ void __launch_bounds__(MXQ_THREADS)

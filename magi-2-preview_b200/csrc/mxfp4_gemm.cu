@@ -257,8 +257,9 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
 }
 
 // The producer and MMA warps share their schedulers with busy epilogue warps, so every
-// instruction of theirs between two asynchronous operations costs tensor time (a loop over the
-// stages with descriptors made on the way ran 803 clocks a stage of 8192^2 x 4096, this form 700).
+// instruction of theirs between two asynchronous operations costs tensor time (8192^2 x 4096: a
+// loop over the stages with descriptors made on the way 120 us, this form 110; and 95 since
+// the scale copies come from the MMA warp and the outputs leave from registers).
 // Hence: the stages are unrolled, so that barriers, descriptors and TMEM columns are constants
 // plus a base; the elected lane and the role are warp-uniform values; all 512 TMEM columns are
 // allocated, so addresses start at 0; and each role reads its next tile's entry a tile ahead.
@@ -288,10 +289,16 @@ __device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int k
 // Wide kernel.  tmT: token rows [R, cols_p/2], box 128 B x 128; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 256.
 //
+// 8192^2 x 4096 with SwiGLU: 95 us, 5.8 PFLOP/s, bound by the MMAs and the waits between a stage's scale copies
+// and its MMAs.  131072 expert rows x 2048 x 1024 with SwiGLU: 139 us, 4.0 PFLOP/s, bound by the
+// epilogue: four stages a tile, and two special-function operations an output are at least 2048
+// clocks a tile, where the MMAs and loads alone take 107 us.
+//
 // One accumulator: its 256 columns leave for registers in about 400 clocks, after which the next tile's MMAs
-// run under the epilogue.  (Two that share 48 columns, the scales in two slots, hid most of the
-// 430, but the barriers they need made both the MMA warp and the epilogue slower: 187 against 165 us
-// for 131072 expert rows x 2048 x 1024, 112 against 109 for 8192^2 x 4096.)
+// run under the epilogue.  Measured and slower (those expert rows; then 8192^2 x 4096): two
+// accumulators sharing 48 columns, the scales in two slots, 187 against 165 us, 112 against 109;
+// pairs of CTAs on one tile (cta_group::2) 252 against 199 with the grouping, 135 against 126 with the quantiser;
+// 8 epilogue warps of 128 columns 213 against 203; SwiGLU in packed pairs 214 against 156.
 template <int OUT, bool SWIGLU>
 __global__ void __launch_bounds__(WideShape::THREADS, 1)
     mx_wide_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
@@ -467,6 +474,9 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
 // XQ (with SPLIT, where a CTA has one item): the type of the up to BN rows of x that the epilogue warps
 // quantise into operand B's stages themselves, before they have outputs to write, instead of a
 // kernel ahead of this one (one token x 4096 x 2048: 8.1 us, 11.3 with the two kernels).
+//
+// Bound by the weights' bytes where there are many (256 rows over 128 experts of 2048 x 1024: 24.5 us, 5.8 TB/s),
+// by latency where there are few: launch, TMEM allocation, the cluster's join and the stores.
 template <int BN, bool SPLIT, int OUT, int XQ>
 __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     mx_flat_kernel(const __grid_constant__ CUtensorMap tmT, const __grid_constant__ CUtensorMap tmW,
@@ -950,8 +960,8 @@ MgPlan mg_plan(int64_t x_rows, int64_t R, int n, int N, int64_t katoms, bool gro
     g.bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 128;
   } else {
     // Above that the wide tile, however few of its 128 rows an expert fills: its 256 weight rows
-    // stream past in 700 clocks a stage, faster than HBM delivers them (128 experts of 2048 x 1024,
-    // 4096 rows: 34 us wide, 45 and 57 flat with 128 and 64 columns).  Flat where the wide tiles
+    // stream past faster than HBM delivers them (128 experts of 2048 x 1024, 4096 rows: 34 us wide, 45
+    // and 57 flat with 128 and 64 columns, grouping included).  Flat where the wide tiles
     // would not reach every SM.
     g.flat = tiles_of(128) * ceil_div(N, 256) < sms;
     g.bn = 128;

@@ -14,7 +14,7 @@ weights that come in this format and for dense layers.  The reference has no cou
 
 Products of two quantised values are exact, sums are fp32, and each output is rounded once.
 All functions enqueue on the current stream of the tensors' device and do not synchronise;
-they have no backward pass, and refuse activations that need one.
+they have no backward pass, and the products refuse inputs that need one.
 """
 from __future__ import annotations
 
@@ -58,7 +58,8 @@ class MXFP4Matrix:
             if t.dtype != torch.uint8 or t.numel() != size or not t.is_contiguous():
                 raise ValueError(f"MXFP4Matrix.{name} must be {size} contiguous uint8 values for {n} x [{rows}, "
                                  f"{self.cols}], got {tuple(t.shape)} {t.dtype}")
-        if self.data.device != self.sf.device or n < 0 or rows < 0 or self.cols < 1 or (n != 1 and not self.batched):
+        if (self.data.device != self.sf.device or n < 0 or rows < 0 or not 0 < self.cols < 1 << 30
+                or (n != 1 and not self.batched)):
             raise ValueError(f"bad MXFP4Matrix: {n} x [{rows}, {self.cols}], batched {self.batched}, on "
                              f"{self.data.device} and {self.sf.device}")
 
@@ -190,7 +191,7 @@ def _product_args(x, bias, activation, n, N, out_dtype, what, row_weights=None):
         raise ValueError(f"swiglu7 pairs columns: {N} weight rows are odd")
     if out_dtype not in _lib.DTYPES:
         raise ValueError(f"out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
-    if torch.is_grad_enabled() and (x.requires_grad or (row_weights is not None and row_weights.requires_grad)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, row_weights, bias)):
         raise ValueError(f"{what} has no backward pass: call it under no_grad or detach its inputs")
     if bias is not None:
         if bias.numel() != n * N or bias.shape[-1] != N:
@@ -260,9 +261,9 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
         y[r] = row_weights[r] * act(Q(x[gather_ids[r]]) W_e^T + bias_e),
         expert_offsets[e] <= r < expert_offsets[e + 1]
 
-    x [T, cols] (fp32, bf16 or fp16); weight [n, N, cols]; expert_offsets int64 (or
-    int32) [n + 1] on the device; gather_ids int32 [R] (default: row r of x itself, R = T); row_weights [R]; bias [n, N];
-    activation, out_dtype and scale_rounding as in ``mxfp4_linear``.
+    x [T, cols] (fp32, bf16 or fp16); weight [n, N, cols]; expert_offsets int64 (or int32) [n + 1]
+    on the device; gather_ids int32 [R] (default: row r of x itself, R = T); row_weights [R]; bias
+    [n, N]; activation, out_dtype and scale_rounding as in ``mxfp4_linear``.
 
     Returns y [R, N] (N/2 with SwiGLU7).  The rows from ``expert_offsets[n]`` on belong to no
     expert: they are 0, or left as they were in ``out`` ([R, N] of the output's type, any row

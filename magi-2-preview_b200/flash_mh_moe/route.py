@@ -279,8 +279,9 @@ def route_experts(
     The weights are differentiable in the logits (first order); the bias only steers the
     selection and gets no gradient.  Forward and backward can be captured into a CUDA graph; as with
     any torch operator, no earlier autograd graph of the same leaf may be alive when a
-    ``backward()`` that accumulates into it is captured (``torch.autograd.grad`` has no such limit).  E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not
-    exceed the experts of ``topk_groups`` groups (``ValueError``).
+    ``backward()`` that accumulates into it is captured (``torch.autograd.grad`` has no such
+    limit).  E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not exceed the experts of
+    ``topk_groups`` groups (``ValueError``).
     """
     score = score_func_name2id_map.get(score_func)
     if score is None:

@@ -280,6 +280,8 @@ def test_expert_linear_no_rows_and_bad_inputs():
                  lambda: mxfp4_expert_linear(x, w, offs, out=torch.zeros(10, 64, device="cuda")[:, ::2]),
                  lambda: mxfp4_expert_linear(x, w, offs, out=torch.zeros(9, 64, dtype=torch.bfloat16, device="cuda")),
                  lambda: mxfp4_expert_linear(x.clone().requires_grad_(True), w, offs),
+                 lambda: mxfp4_expert_linear(x, w, offs, bias=torch.zeros(3, 64, device="cuda", requires_grad=True)),
+                 lambda: mxfp4_expert_linear(x, w, offs, row_weights=torch.ones(10, device="cuda", requires_grad=True)),
                  lambda: mxfp4_expert_linear(x, w, offs, gather_ids=ids.long()),
                  lambda: mxfp4_expert_linear(x, w, offs.float()),
                  lambda: mxfp4_expert_linear(x, w, offs, activation="gelu")]:

@@ -57,7 +57,7 @@ def test_matrix_refuses_sizes_it_does_not_hold():
     d, s = torch.zeros(1, 5, 64, dtype=torch.uint8), torch.zeros(1, 512, dtype=torch.uint8)
     m = MXFP4Matrix(d, s, 5, 100, 1, False)
     assert m.to("cpu").shape == (5, 100)
-    for bad in [(d, s, 6, 100, 1, False), (d, s, 5, 129, 1, False), (d, s[:, :100], 5, 100, 1, False),
+    for bad in [(d[:0], s[:0], 5, 0, 1, False), (d[:0], s[:0], 0, 1 << 30, 1, False), (d, s, 6, 100, 1, False), (d, s, 5, 129, 1, False), (d, s[:, :100], 5, 100, 1, False),
                 (d.float(), s, 5, 100, 1, False), (d, s, 5, 100, 2, True), (d.transpose(1, 2), s, 5, 100, 1, False),
                 (torch.zeros(2, 5, 64, dtype=torch.uint8), torch.zeros(2, 512, dtype=torch.uint8), 5, 100, 2, False)]:
         with pytest.raises(ValueError):
