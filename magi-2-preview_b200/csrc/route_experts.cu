@@ -204,13 +204,16 @@ __host__ __device__ constexpr int fwd_scratch_bytes(int E, int npl, int rpw, boo
 // themselves (no bias) are exact: 16-bit ones fit above the id bits, so their keys are too.
 //
 // Bound by instructions and the latency of the K dependent maxima, not by the 2 or 4 B a logit read: that is
-// why up to four rows share a warp's reductions.  196608 rows of 256 fp32 logits, top-6 of sigmoid
-// + bias: 108 us, 2.0 TB/s (222 with a row a warp and the ids reduced beside the values);
-// 16381 rows of 128, softmax top-8: 19 us; 16396 rows of 160 in 8 groups: 35 us.  A full fp32 count of the
-// row's candidates before the 64-bit selection saved none of it (109 against 108 us).
-template <int DT, int NPL, int RPW, bool GROUPED>
-__global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 4)
-    route_experts_kernel(const __grid_constant__ RouteArgs a, bool vec, unsigned per_magic, float* __restrict__ weights, int64_t* __restrict__ idx, float* __restrict__ saved) {
+// why up to four rows share a warp's reductions, and why kernels of four rows have the score function and
+// the presence of a bias (SCORE, BIAS; -1: read from the arguments) as constants.  196608 rows of 256 fp32
+// logits, top-6 of sigmoid + bias: 88 us, 2.4 TB/s (108 with the two read from the arguments and a block
+// more a SM; 222 with a row a warp and the ids reduced beside the values); 16381 rows of 128, softmax
+// top-8: 16 us (19); 16396 rows of 160 in 8 groups: 30 us (35).  A full fp32 count of the row's
+// candidates before the 64-bit selection saved none of it (109 against 108 us).
+template <int DT, int NPL, int RPW, bool GROUPED, int SCORE, int BIAS>
+__global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? (SCORE < 0 ? 9 : 8) : NPL <= 16 ? 6 : 4)
+    route_experts_kernel(const __grid_constant__ RouteArgs a, bool vec, unsigned per_magic, float* __restrict__ weights,
+                         int64_t* __restrict__ idx, float* __restrict__ saved) {
   pdl_wait();
   pdl_trigger();
   using T = typename MxType<DT>::T;
@@ -222,8 +225,9 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
   const unsigned rows = (unsigned)(a.H * a.S), row0 = (blockIdx.x * RE_WARPS + warp) * RPW;
   if (row0 >= rows) return;
   const int n_rows = (int)min((unsigned)RPW, rows - row0), mine_r = lane / SEG, rank = lane % SEG;
+  const bool softmax = SCORE < 0 ? a.score_func == 0 : SCORE == 0, biased = BIAS < 0 ? a.bias != nullptr : BIAS == 1;
   const int E = a.E, K = a.K, e0 = lane * NPL, G = a.groups;
-  const bool exact = DT != DT_F32 && !a.bias;
+  const bool exact = DT != DT_F32 && !biased;
   const int bytes = fwd_scratch_bytes(E, NPL, RPW, GROUPED);
   double* scratch = smd + (size_t)warp * (bytes / 8);
   unsigned* lists = reinterpret_cast<unsigned*>(scratch);         // [RPW][NPL + 1][32]
@@ -246,7 +250,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
       s = 0;
       ++h;
     }
-    if (a.bias && (r == 0 || s == 0)) {
+    if (biased && (r == 0 || s == 0)) {
       load_chunk<float, NPL>(a.bias + (int64_t)h * E, e0, E, vec, 0.f, b);
       float probe = 0.f;
 #pragma unroll
@@ -261,14 +265,13 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
     list[0] = 0;                                                  // for a row without a choice
     if (a.token_mask && !a.token_mask[h * a.mask_stride_h + s]) continue;
     const bool mine_row = mine_r == r;
-    const bool bias = a.bias != nullptr;
     // infinities and NaN make a product with 0 that is not 0; lanes that reach over E count too
     float probe = 0.f;
 #pragma unroll
     for (int j = 0; j < NPL; ++j) probe = fmaf(x[j], 0.f, probe);
     const bool special = e0 < E && !(probe == 0.f);
     float m = 0.f, tol0 = 0x1p-20f;
-    if (a.score_func == 0) {
+    if (softmax) {
       m = x[0];
 #pragma unroll
       for (int j = 1; j < NPL; ++j) m = fmaxf(m, x[j]);
@@ -283,9 +286,9 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
       if (m == -INFINITY) continue;                               // no expert is left
     }
     unsigned key[NPL];
-    if (bias || GROUPED || a.score_func == 0) {
+    if (biased || GROUPED || softmax) {
       float v[NPL];
-      if (a.score_func == 0) {
+      if (softmax) {
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < NPL; ++j) {
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
           sum_l = sum;
         }
         tol0 = smax * 0x1p-17f;
-        if (bias || GROUPED) {
+        if (biased || GROUPED) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j) v[j] *= smax;
         }
@@ -307,8 +310,8 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
 #pragma unroll
         for (int j = 0; j < NPL; ++j) v[j] = rcp_approx(1.f + ex2_approx(x[j] * -LOG2E));
       }
-      if (bias || GROUPED) {
-        if (bias) {
+      if (biased || GROUPED) {
+        if (biased) {
 #pragma unroll
           for (int j = 0; j < NPL; ++j) v[j] += b[j];
         }
@@ -319,7 +322,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
 #pragma unroll
           for (int j = 0; j < NPL; ++j) {
             if (v[j] != v[j]) key[j] = order_key(-FLT_MAX);
-            if (x[j] == -INFINITY || (bias && b[j] == -INFINITY)) key[j] = 0;
+            if (x[j] == -INFINITY || (biased && b[j] == -INFINITY)) key[j] = 0;
           }
         }
       }
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
       if (best) close |= mine_row && !(key_value(last & ~63u) - key_value(best | 63u) > 4.f * tol0 + 0x1p-21f * mag);
       __syncwarp();
     }
-    if (!bias) {
+    if (!biased) {
       if (special) {
 #pragma unroll
         for (int j = 0; j < NPL; ++j)
@@ -438,21 +441,21 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
   h = row / (unsigned)a.S;
   s = row - h * (unsigned)a.S;
   const T* lg = static_cast<const T*>(a.logits) + h * a.stride_h + s * a.stride_s;
-  const float* bias = a.bias ? a.bias + (int64_t)h * E : nullptr;
+  const float* bias = biased ? a.bias + (int64_t)h * E : nullptr;
   int mine = mine_key > ID ? (int)(ID - (mine_key & ID)) : -1;
   float x = 0.f, p = 0.f, b_mine = 0.f;
   auto score = [&] {
     p = 0.f;
     if (mine >= 0) {
       x = mx_to_f32(lg[mine]);
-      p = a.score_func == 0 ? __fdividef(expf(x - m_l), sum_l) : __fdividef(1.f, 1.f + expf(-x));
+      p = softmax ? __fdividef(expf(x - m_l), sum_l) : __fdividef(1.f, 1.f + expf(-x));
     }
   };
   score();
   if (!exact) {
-    if (bias && mine >= 0) b_mine = bias[mine];
-    const float v = bias ? p + b_mine : x;
-    const float tol = bias ? tol_l + 0x1p-22f * fabsf(v) : 0.f;
+    if (biased && mine >= 0) b_mine = bias[mine];
+    const float v = biased ? p + b_mine : x;
+    const float tol = biased ? tol_l + 0x1p-22f * fabsf(v) : 0.f;
     const float v1 = __shfl_down_sync(FULL, v, 1), x1 = __shfl_down_sync(FULL, x, 1), b1 = __shfl_down_sync(FULL, b_mine, 1);
     const bool next = __shfl_down_sync(FULL, mine, 1) >= 0;
     if (mine >= 0) {
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? 9 : NPL <= 16 ? 6 : 
     const int64_t o = (int64_t)row * K + rank;
     weights[o] = w * a.route_scale;
     idx[o] = mine;
-    if (saved) saved[o] = a.score_func == 0 ? p : x;
+    if (saved) saved[o] = softmax ? p : x;
   }
 }
 
@@ -611,12 +614,12 @@ int rows_per_warp(int64_t rows, int K) {
   return rpw;
 }
 
-template <int DT, int NPL, int RPW, bool GROUPED>
+template <int DT, int NPL, int RPW, bool GROUPED, int SCORE = -1, int BIAS = -1>
 cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
   const int64_t rows = (int64_t)a.H * a.S;
   const unsigned grid = (unsigned)((rows + RE_WARPS * RPW - 1) / (RE_WARPS * RPW));
   const size_t smem = (size_t)RE_WARPS * fwd_scratch_bytes(a.E, NPL, RPW, GROUPED);
-  auto kernel = route_experts_kernel<DT, NPL, RPW, GROUPED>;
+  auto kernel = route_experts_kernel<DT, NPL, RPW, GROUPED, SCORE, BIAS>;
   if (smem > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
@@ -625,8 +628,8 @@ cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* sav
                    (!a.bias || chunks_aligned(a.bias, a.E, 0, a.E, 4, NPL));
   // e / per = e * ceil(2^20 / per) >> 20 for e < 1024
   const unsigned per = (unsigned)(a.E / a.groups), magic = ((1u << 20) + per - 1) / per;
-  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL, RPW, GROUPED>), grid, RE_WARPS * 32, smem, st, a, vec, magic, weights,
-                   idx, saved);
+  MHMOE_LAUNCH_PDL((route_experts_kernel<DT, NPL, RPW, GROUPED, SCORE, BIAS>), grid, RE_WARPS * 32, smem, st, a, vec,
+                   magic, weights, idx, saved);
   return cudaGetLastError();
 }
 
@@ -634,7 +637,13 @@ template <int DT, int NPL, bool GROUPED>
 cudaError_t run_fwd(const RouteArgs& a, float* weights, int64_t* idx, float* saved, cudaStream_t st) {
   if constexpr (NPL <= 8) {
     const int rpw = rows_per_warp((int64_t)a.H * a.S, a.K);
-    if (rpw == 4) return run_fwd<DT, NPL, 4, GROUPED>(a, weights, idx, saved, st);
+    if (rpw == 4) {                                               // many rows: one kernel a score and bias
+      if (a.score_func == 0)
+        return a.bias ? run_fwd<DT, NPL, 4, GROUPED, 0, 1>(a, weights, idx, saved, st)
+                      : run_fwd<DT, NPL, 4, GROUPED, 0, 0>(a, weights, idx, saved, st);
+      return a.bias ? run_fwd<DT, NPL, 4, GROUPED, 1, 1>(a, weights, idx, saved, st)
+                    : run_fwd<DT, NPL, 4, GROUPED, 1, 0>(a, weights, idx, saved, st);
+    }
     if (rpw == 2) return run_fwd<DT, NPL, 2, GROUPED>(a, weights, idx, saved, st);
   }
   return run_fwd<DT, NPL, 1, GROUPED>(a, weights, idx, saved, st);
