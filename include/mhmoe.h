@@ -13,7 +13,9 @@
  *
  * Kernels that wait on on-chip barriers give up after `timeout_ns` (0 selects
  * the default of 2 s) and record MHMOE_ERR_TIMEOUT in the optional device word
- * `dev_status` (int32, caller-zeroed); the host reads it when convenient.
+ * `dev_status` (int32, caller-zeroed); the host reads it when convenient.  Such a
+ * status ends the waits that poll the same word; MHMOE_ERR_ARGS, which kernels record
+ * where they clip, skip or read zeros and go on, ends none and is written over by it.
  *
  * Layout conventions (row-major unless stated):
  *   x            bf16 [S, H, dh]   strides in elements; dh stride must be 1

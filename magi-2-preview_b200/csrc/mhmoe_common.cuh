@@ -38,6 +38,17 @@ __device__ __forceinline__ void record_error(int* err, int code) {
   if (err) atomicCAS(err, 0, code);
 }
 
+// A wait that gave up is recorded over an argument error (MHMOE_ERR_ARGS), which is recoverable: the kernel
+// that records one clips, skips or reads zeros, and goes on.  Hence that status also ends no wait
+// of this or a later launch; any other does.
+__device__ __forceinline__ void record_gave_up(int* err, int code) {
+  if (err && atomicCAS(err, 0, code) == MHMOE_ERR_ARGS) atomicCAS(err, MHMOE_ERR_ARGS, code);
+}
+__device__ __forceinline__ bool ends_waits(const int* err) {
+  const int s = ld_volatile_i32(err);
+  return s != MHMOE_OK && s != MHMOE_ERR_ARGS;
+}
+
 __device__ __forceinline__ bool elect_one() {
   uint32_t pred = 0;
   asm volatile(
@@ -87,8 +98,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// Bounded wait.  Returns false (and records `code`) on timeout or when another
-// role of this grid already recorded an error.
+// Bounded wait.  Returns false on timeout (recording `code`) or when another role already
+// recorded that it gave up.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* err, int code,
                                           uint64_t timeout_ns) {
   if (mbar_try_wait(bar, parity)) return true;
@@ -96,9 +107,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* er
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((i & 255u) == 0) {
-      if (err && ld_volatile_i32(err) != 0) return false;
+      if (err && ends_waits(err)) return false;
       if (globaltimer_ns() - t0 > timeout_ns) {
-        record_error(err, code);
+        record_gave_up(err, code);
         return false;
       }
     }
@@ -121,9 +132,9 @@ __device__ __forceinline__ bool flag_wait_geq(const int* flag, int expected, int
     asm volatile("ld.acquire.sys.global.s32 %0, [%1];" : "=r"(v) : "l"(flag) : "memory");
     if (v >= expected) return true;
     if ((i & 63u) == 63u) {
-      if (err && ld_volatile_i32(err) != 0) return false;
+      if (err && ends_waits(err)) return false;
       if (globaltimer_ns() - t0 > timeout_ns) {
-        record_error(err, code);
+        record_gave_up(err, code);
         return false;
       }
     }

@@ -109,6 +109,28 @@ __device__ __forceinline__ MgTile mg_tile(const MgParams& p, const int4& v) {
   return t;
 }
 
+// Bounded wait of one role.  A role that gives up tells the others of its CTA through `gave_up` in shared
+// memory and the host through the status word.  What that word held before ends no wait: it is kept
+// from call to call, and an earlier launch's error is not this one's.
+__device__ __forceinline__ bool mg_wait(uint32_t bar, uint32_t parity, uint32_t gave_up, int* status,
+                                        uint64_t timeout_ns) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t i = 1;; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 0) {
+      int left;
+      asm volatile("ld.volatile.shared::cta.s32 %0, [%1];" : "=r"(left) : "r"(gave_up) : "memory");
+      if (left) return false;
+      if (globaltimer_ns() - t0 > timeout_ns) {
+        asm volatile("st.volatile.shared::cta.s32 [%0], %1;" ::"r"(gave_up), "r"(1) : "memory");
+        record_gave_up(status, MHMOE_ERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
 template <int OUT>
 __device__ __forceinline__ uint32_t mg_pack16(float a, float b) {
   if constexpr (OUT == DT_F16) {
@@ -320,7 +342,8 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
   uint64_t* tempty_bar = tfull_bar + 1;
   uint64_t* drain_bar = tempty_bar + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
-  static_assert((2 * STAGES + 3) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  const uint32_t gave_up = smem_u32(tmem_slot + 1);
+  static_assert((2 * STAGES + 3) * 8 + 8 <= MG_MISC_BYTES, "barriers");
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0);   // known to be uniform
   const int lane = threadIdx.x & 31;
@@ -332,6 +355,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     mbar_init(smem_u32(tfull_bar), 1);
     mbar_init(smem_u32(tempty_bar), EPW);
     mbar_init(smem_u32(drain_bar), 1);
+    tmem_slot[1] = 0;                              // gave_up
     fence_mbar_init();
     tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
@@ -370,7 +394,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
         second = wt * 2 + 1 < (int)wblk;
         if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       }
-      if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mg_wait(smem_u32(&empty_bar[s]), phase ^ 1, gave_up, p.status, timeout)) return false;
       if (one) {
         const uint32_t fb = smem_u32(&full_bar[s]);
         const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;      // atoms of this stage
@@ -398,8 +422,8 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
     const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
     // A stage's scale slot in TMEM is free when the stage is: both wait for the MMAs of the round before.
     mg_for_stages<STAGES, true>(t0, total, step, 0, n_kblk, [&](int, int kb, int s, uint32_t phase) {
-      if (kb == 0 && !mbar_wait(smem_u32(tempty_bar), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
-      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (kb == 0 && !mg_wait(smem_u32(tempty_bar), acc_phase ^ 1, gave_up, p.status, timeout)) return false;
+      if (!mg_wait(smem_u32(&full_bar[s]), phase, gave_up, p.status, timeout)) return false;
       tc_fence_after();
       const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
       const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8;
@@ -438,7 +462,7 @@ __global__ void __launch_bounds__(WideShape::THREADS, 1)
       const int wt = t % p.n_wt;
       const MgTile tile = mg_tile<S::SLOT>(p, next);
       if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
-      if (!mbar_wait(smem_u32(tfull_bar), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
+      if (!mg_wait(smem_u32(tfull_bar), acc_phase, gave_up, p.status, timeout)) break;
       acc_phase ^= 1;
       tc_fence_after();
       uint32_t r[64];
@@ -498,7 +522,8 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
   uint64_t* tempty_bar = tfull_bar + NACC;     // [NACC]
   uint64_t* drain_bar = tempty_bar + NACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
-  static_assert((2 * STAGES + 2 * NACC + 1) * 8 + 4 <= MG_MISC_BYTES, "barriers");
+  const uint32_t gave_up = smem_u32(tmem_slot + 1);
+  static_assert((2 * STAGES + 2 * NACC + 1) * 8 + 8 <= MG_MISC_BYTES, "barriers");
   static_assert(XQ < 0 || (SPLIT && BN <= 32 && EPW == 4), "a stage of rows is quantised by 128 threads");
   static_assert(!SPLIT || BN * 128 * 4 <= STAGES * MG_A_BYTES, "partial sums lie over operand A's stages");
 
@@ -514,6 +539,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       mbar_init(smem_u32(&tempty_bar[a]), EPW);
     }
     mbar_init(smem_u32(drain_bar), 1);
+    tmem_slot[1] = 0;                              // gave_up
     fence_mbar_init();
     if (XQ < 0) tma_prefetch_desc(&tmT);
     tma_prefetch_desc(&tmW);
@@ -558,7 +584,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
         sf_w = p.sf_w + ((uint64_t)tile.e * wblk + wt) * p.katoms * 512;
         if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       }
-      if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mg_wait(smem_u32(&empty_bar[s]), phase ^ 1, gave_up, p.status, timeout)) return false;
       if (one) {
         const uint32_t fb = smem_u32(&full_bar[s]);
         const uint32_t sfn = min(2u, p.katoms - 2 * kb) * 512;      // atoms of this stage
@@ -586,9 +612,9 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
     const uint64_t sa0 = sdesc_sf_chunk(smem_u32(sSFA)), sb0 = sdesc_sf_chunk(smem_u32(sSFB));
     // A stage's scale slot in TMEM is free when the stage is: both wait for the MMAs of the round before.
     mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
-      if (kb == kb0 && !mbar_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout))
+      if (kb == kb0 && !mg_wait(smem_u32(&tempty_bar[acc]), acc_phase ^ 1, gave_up, p.status, timeout))
         return false;
-      if (!mbar_wait(smem_u32(&full_bar[s]), phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+      if (!mg_wait(smem_u32(&full_bar[s]), phase, gave_up, p.status, timeout)) return false;
       tc_fence_after();
       const uint64_t a_d = a0 + s * (MG_A_BYTES >> 4), b_d = b0 + s * (S::B_BYTES >> 4);
       const uint32_t tsfa = S::SF_COL0 + s * S::SF_COLS, tsfb = tsfa + 8, d = acc * BN;
@@ -630,7 +656,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       const int tid = threadIdx.x - 64, chunk = tid & 15;
       const uint32_t mask = 0xffu << (lane & 24);
       mg_for_stages<STAGES, false>(t0, total, step, kb0, kb1, [&](int, int kb, int s, uint32_t phase) {
-        if (!mbar_wait(smem_u32(&empty_bar[s]), phase ^ 1, p.status, MHMOE_ERR_TIMEOUT, timeout)) return false;
+        if (!mg_wait(smem_u32(&empty_bar[s]), phase ^ 1, gave_up, p.status, timeout)) return false;
         const int c0 = kb * MG_BK + chunk * 16;
 #pragma unroll
         for (int row = tid >> 4; row < BN; row += 8) {
@@ -662,7 +688,7 @@ __global__ void __launch_bounds__(FlatShape<BN>::THREADS, 1)
       if (t + step < total) next = mg_fetch(p, (t + step) / p.n_wt);
       const int n0 = wt * 128 + q * 32;
       const float b = p.bias && n0 + lane < p.N ? __ldg(p.bias + (int64_t)tile.e * p.N + n0 + lane) : 0.f;
-      if (!mbar_wait(smem_u32(&tfull_bar[acc]), acc_phase, p.status, MHMOE_ERR_TIMEOUT, timeout)) break;
+      if (!mg_wait(smem_u32(&tfull_bar[acc]), acc_phase, gave_up, p.status, timeout)) break;
       tc_fence_after();
       const uint32_t taddr = ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN);
       for (int j0 = part * NC; j0 < BN && j0 < tile.rows; j0 += NC * (EPW / 4)) {
