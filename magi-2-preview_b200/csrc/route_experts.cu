@@ -5,7 +5,7 @@
 //   key   = score + bias, or l itself without a bias (both scores are monotone in l)
 //   group score = sum of the two largest unmasked (score + bias) of a group; the `keep` best
 //   groups stay; the K largest keys among them are chosen, equal keys to the lower id
-//   w = scale * score / max(sum of the chosen scores, eps)  (or scale * score)
+//   w = scale * score / max(sum of the chosen scores, eps)  (or scale * score); 0 without an expert
 // The selection is that of 64-bit keys: it does not depend on how 32-bit scores round.
 //
 // Backward, from the weights' gradient g (times scale) and the chosen scores p:
@@ -484,7 +484,9 @@ __global__ void __launch_bounds__(RE_WARPS * 32, NPL <= 8 ? (SCORE < 0 ? 9 : 8) 
     float n = p;
     #pragma unroll
     for (int o = SEG / 2; o > 0; o >>= 1) n += __shfl_xor_sync(FULL, n, o);
-    w = __fdividef(p, n != n ? n : fmaxf(n, a.norm_eps));
+    // a slot without an expert weighs 0 whatever the divisor is, and so does all of a sum of 0 without an eps
+    const float d = n != n ? n : fmaxf(n, a.norm_eps);
+    w = mine >= 0 && d != 0.f ? __fdividef(p, d) : 0.f;
   }
   if (live) {
     const int64_t o = (int64_t)row * K + rank;
@@ -532,14 +534,21 @@ __global__ void __launch_bounds__(RE_WARPS * 32)
     for (int o = seg / 2; o > 0; o >>= 1) v += __shfl_xor_sync(FULL, v, o);
     return v;
   };
-  float ds = g;
+  float ds = g, unscale = 1.f;
   bool cancels = false;                                           // the softmax's common term is 0
   if (a.route_norm) {
-    const float n = seg_sum(p), gp = seg_sum(g * p);
-    const float den = n != n ? n : fmaxf(n, a.norm_eps);
+    const float n = seg_sum(p);
+    float den = n != n ? n : fmaxf(n, a.norm_eps);
     cancels = n > a.norm_eps;
+    if (den < 0x1p-64f) {           // g / den alone could overflow: p and den times 2^64, ds over it
+      unscale = 0x1p-64f;
+      p *= 0x1p64f;
+      den = den < FLT_MIN ? 0.f : den * 0x1p64f;                  // scores below FLT_MIN counted as 0
+    }
+    const float gp = seg_sum(g * p);
     ds = __fdiv_rn(g, den);
     if (cancels) ds = __fdiv_rn(g - __fdiv_rn(gp, den), den);
+    if (den == 0.f) ds = 0.f;                                     // the weights were 0
   }
   const bool dense_row = a.score_func == 0 && !cancels;
   const float dot = seg_sum(has && dense_row ? ds * p : 0.f);
@@ -590,7 +599,7 @@ __global__ void __launch_bounds__(RE_WARPS * 32)
     }
   }
   __syncwarp();
-  if (has) mx_store(dl + (int64_t)row * E + id, a.score_func == 1 ? ds * p * q : p * (ds - dot));
+  if (has) mx_store(dl + (int64_t)row * E + id, a.score_func == 1 ? ds * p * q : p * (ds - dot * unscale));
 }
 
 // Experts a lane: the smallest power of two that covers E with 32 lanes.

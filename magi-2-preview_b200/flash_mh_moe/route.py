@@ -274,7 +274,8 @@ def route_experts(
     * ``token_mask`` (bool [S] or [H, S]): tokens that are False get -1 and 0 throughout, and
       their logits (NaN included) are not looked at;
     * weights are ``route_scale * s / max(sum of the chosen s, norm_eps)``, or
-      ``route_scale * s`` without ``route_norm``.
+      ``route_scale * s`` without ``route_norm``.  With ``norm_eps = 0`` sigmoid scores below the
+      smallest normal fp32 number count as 0, and over a sum of 0 weights and gradients are 0.
 
     The weights are differentiable in the logits (first order); the bias only steers the
     selection and gets no gradient.  Forward and backward can be captured into a CUDA graph; as with
