@@ -11,6 +11,7 @@ import os
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 _PKG_ROOT = Path(__file__).resolve().parent.parent
 LIB_PATH = Path(os.environ.get("MHMOE_LIB", _PKG_ROOT / "lib" / "libmhmoe.so"))
@@ -149,6 +150,15 @@ def require_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if t is not None and not t.is_cuda:
             raise ValueError("flash_mh_moe (B200) needs CUDA tensors; there is no CPU path")
+
+
+def require_no_tangent(what: str, *ts) -> None:
+    """Refuse dual tensors of forward-mode differentiation: a kernel reads their primals alone, and a
+    result without a tangent would stand for a derivative of zero."""
+    if _forward_ad._current_level >= 0:
+        for t in ts:
+            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{what} has no forward-mode derivative: pass tensors without a tangent")
 
 
 _status: dict[int, torch.Tensor] = {}

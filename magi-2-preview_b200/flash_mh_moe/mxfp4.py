@@ -14,7 +14,7 @@ weights that come in this format and for dense layers.  The reference has no cou
 
 Products of two quantised values are exact, sums are fp32, and each output is rounded once.
 All functions enqueue on the current stream of the tensors' device and do not synchronise;
-they have no backward pass, and the products refuse inputs that need one.
+they have no backward pass (nor a forward-mode derivative), and the products refuse inputs that need one.
 """
 from __future__ import annotations
 
@@ -213,6 +213,7 @@ def mxfp4_linear(x: torch.Tensor | MXFP4Matrix, weight: MXFP4Matrix, bias: torch
     into N/2 outputs: min(g, 7) sigmoid(1.702 min(g, 7)) (clamp(u, -7, 7) + 1).  The result has
     ``out_dtype`` (default: x's type, bf16 for an MXFP4 x)."""
     rounding = _check_rounding(scale_rounding)
+    _lib.require_no_tangent("mxfp4_linear", x, bias)
     quantized = isinstance(x, MXFP4Matrix)
     if quantized:
         _check_matrix(x, "x")
@@ -271,6 +272,7 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
     outside [0, T) reads as a row of zeros; both record an error that
     ``_lib.check_device_status`` raises."""
     rounding = _check_rounding(scale_rounding)
+    _lib.require_no_tangent("mxfp4_expert_linear", x, row_weights, bias, out)
     _check_float(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be [T, cols], got {tuple(x.shape)}")

@@ -277,7 +277,8 @@ def route_experts(
       ``route_scale * s`` without ``route_norm``.  With ``norm_eps = 0`` sigmoid scores below the
       smallest normal fp32 number count as 0, and over a sum of 0 weights and gradients are 0.
 
-    The weights are differentiable in the logits (first order); the bias only steers the
+    The weights are differentiable in the logits (first order, backward mode; logits with a
+    forward-mode tangent are refused); the bias only steers the
     selection and gets no gradient.  Forward and backward can be captured into a CUDA graph; as with
     any torch operator, no earlier autograd graph of the same leaf may be alive when a
     ``backward()`` that accumulates into it is captured (``torch.autograd.grad`` has no such
@@ -289,6 +290,7 @@ def route_experts(
         raise ValueError(f"Unknown score_func: {score_func}")
     if logits.dim() != 3 or logits.dtype not in _lib.DTYPES:
         raise ValueError(f"logits must be [H, S, E] in fp32, bf16 or fp16, got {tuple(logits.shape)} {logits.dtype}")
+    _lib.require_no_tangent("route_experts", logits)
     _lib.require_cuda(logits)
     H, S, E = logits.shape
     bias = mask = None
