@@ -76,7 +76,8 @@ class MultiHeadMoELayerConfig:
     split_merge_intermediate_size: Optional[int]
     moe_config: MoEConfig
     # "bf16": the split and merge linears are library GEMMs; "mxfp4": their weights are held in MXFP4
-    # and the activations quantised on the way (flash_mh_moe.mxfp4; no reference key)
+    # and the activations quantised on the way (flash_mh_moe.mxfp4; no reference key).  For inference:
+    # a backward pass through the layer raises, forward-mode tangents are refused
     linear_format: str = "bf16"
 
 
@@ -175,6 +176,20 @@ def create_linear(in_features: int, out_features: int, num_layers: int = 1, num_
     """magi2_preview.py:672-698."""
     return CustomGroupedLinear(in_features, out_features, num_experts, num_patterns, num_layers, bias, device,
                                dtype)
+
+
+class _NoBackward(torch.autograd.Function):
+    """``out`` marked as depending on ``inputs``: a backward pass through it raises."""
+
+    @staticmethod
+    def forward(ctx, out, *inputs):
+        ctx.mark_dirty(out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("MultiHeadMoELayer with linear_format='mxfp4' has no backward pass: its split and merge "
+                           "weights are read in their packed form")
 
 
 class MultiHeadMoELayer(nn.Module):
@@ -292,13 +307,19 @@ class MultiHeadMoELayer(nn.Module):
         sizes, cu = group_layout(modality_dispatcher, x.shape[0], self.config.num_modality, x.device)
         norm_output = self.pre_norm(x, cu_groups=cu)
         mx = self.config.linear_format == "mxfp4"
+        if mx:
+            differentiable = (hidden_states, self.split_linear.weight, self.merge_linear.weight)
+            _lib.require_no_tangent("MultiHeadMoELayer with linear_format='mxfp4'", *differentiable)
         split = (mxfp4_linear(norm_output, self._linear_mxfp4("split_linear")) if mx
                  else F.linear(norm_output, self.split_linear.weight))
         moe_out = self.moe_mlp(split)
         shared = self._shared_expert_forward(norm_output, sizes)
         if mx:                                    # added in fp32, rounded once
             merged = mxfp4_linear(moe_out, self._linear_mxfp4("merge_linear"), out_dtype=torch.float32)
-            return merged.add_(shared).to(shared.dtype).view(shape)
+            out = merged.add_(shared).to(shared.dtype)
+            if torch.is_grad_enabled() and any(t.requires_grad for t in differentiable):
+                out = _NoBackward.apply(out, *differentiable)
+            return out.view(shape)
         # merge_linear(moe_out) + shared in one GEMM (accumulating onto the shared output)
         out = torch.addmm(shared, moe_out, self.merge_linear.weight.t())
         return out.view(shape)
