@@ -227,7 +227,8 @@ class MultiHeadMoELayer(nn.Module):
         self._shared_packed = None
         self._shared_key = None
         self._routing_cache: dict = {}
-        self._linear_packed: dict = {}
+        self._linear_packed: dict = {}             # name -> (key, MXFP4Matrix, handle of the packing stream)
+        self._linear_captured: list = []           # packed weights that a captured graph reads
 
     # ── shared experts as an NVFP4 expert set: expert 0 = shared, expert 1 + m = modality m ──
     def _shared_params(self):
@@ -291,14 +292,32 @@ class MultiHeadMoELayer(nn.Module):
         return y.view(S, d)
 
     def _linear_mxfp4(self, name: str) -> MXFP4Matrix:
-        """The MXFP4 form of ``split_linear`` / ``merge_linear``, packed again when its parameter changes."""
+        """The MXFP4 form of ``split_linear`` / ``merge_linear``, packed again when its parameter changes.
+
+        The host waits once for a packing that is kept, so that any stream may read it.  A stream other
+        than the packing one is recorded as a reader, and what a graph captured stays allocated: an
+        update frees neither under its reader.  In a capture nothing runs yet, so a packing there
+        belongs to the graph and is not kept."""
         w = getattr(self, name).weight
         key = ((w, w.data_ptr(), w._version),)
+        with torch.cuda.device(w.device):
+            capturing = torch.cuda.is_current_stream_capturing()
+            stream = torch.cuda.current_stream()
         hit = self._linear_packed.get(name)
         if hit is None or not _same_key(hit[0], key):
-            hit = (key, mxfp4_quantize(w))
-            self._linear_packed[name] = hit
-        return hit[1]
+            m = mxfp4_quantize(w)
+            if not capturing:
+                stream.synchronize()
+                self._linear_packed[name] = (key, m, stream.cuda_stream)
+            return m
+        m = hit[1]
+        if capturing:
+            if not any(c is m for c in self._linear_captured):
+                self._linear_captured.append(m)
+        elif stream.cuda_stream != hit[2]:
+            m.data.record_stream(stream)
+            m.sf.record_stream(stream)
+        return m
 
     def forward(self, hidden_states: torch.Tensor, modality_dispatcher=None) -> torch.Tensor:
         _lib.require_cuda(hidden_states)
