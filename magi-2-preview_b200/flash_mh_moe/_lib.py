@@ -169,7 +169,22 @@ def device_status(device: torch.device) -> torch.Tensor:
     idx = device.index if device.index is not None else torch.cuda.current_device()
     t = _status.get(idx)
     if t is None:
-        t = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        dev = torch.device("cuda", idx)
+        with torch.cuda.device(idx):
+            if torch.cuda.is_current_stream_capturing():
+                # not cleared by the graph: the word has to be 0 before any replay, and a replay may not clear what
+                # was recorded since
+                t = torch.empty(1, dtype=torch.int32, device=dev)
+                for _ in range(64):                # streams come from a pool: one that takes no part in the capture
+                    with torch.cuda.stream(torch.cuda.Stream(dev)):
+                        if not torch.cuda.is_current_stream_capturing():
+                            t.zero_()
+                            break
+                else:
+                    raise MHMoEError("no stream outside of the capture to clear the device status word on")
+            else:
+                t = torch.zeros(1, dtype=torch.int32, device=dev)
+                torch.cuda.current_stream().synchronize()      # 0 for every stream from here on
         _status[idx] = t
     return t
 
