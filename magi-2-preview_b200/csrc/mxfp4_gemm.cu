@@ -829,14 +829,16 @@ __device__ __forceinline__ void mg_list_tiles(const MgGroup& p) {
       before += w < warp ? wsum[w] : 0;
       all += wsum[w];
     }
-    const int at = base + before + inc - cnt;
+    const int64_t at = (int64_t)base + before + inc - cnt;
     const int slot0 = (int)(a / p.slot_rows) + e;
     for (int j = 0; j < cnt && at + j < p.max_tiles; ++j)
       p.tiles[at + j] = make_int4(e, (int)a + j * p.slot_rows, min(p.slot_rows, rows - j * p.slot_rows), slot0 + j);
-    base += all;
+    // Offsets that decrease can count the rows many times over: such a sum is above max_tiles in this round
+    // (256 experts of up to 2^23 tiles, every other one, fit 31 bits) and stays there.
+    base = (int)min((int64_t)base + all, (int64_t)p.max_tiles);
     __syncthreads();
   }
-  if (threadIdx.x == 0) *p.n_tiles = min(base, p.max_tiles);
+  if (threadIdx.x == 0) *p.n_tiles = base;
   if (bad) record_error(p.status, MHMOE_ERR_ARGS);
 }
 
