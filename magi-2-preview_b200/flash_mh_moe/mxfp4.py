@@ -184,14 +184,14 @@ def mxfp4_dequantize(m: MXFP4Matrix, dtype: torch.dtype = torch.float32) -> torc
     return out
 
 
-def _product_args(x, bias, activation, n, N, out_dtype, what, row_weights=None):
+def _product_args(x, bias, activation, n, N, out_dtype, what, row_weights=None, out=None):
     if activation not in _ACTIVATION:
         raise ValueError(f"activation must be None or 'swiglu7', got {activation!r}")
     if activation and N % 2:
         raise ValueError(f"swiglu7 pairs columns: {N} weight rows are odd")
     if out_dtype not in _lib.DTYPES:
         raise ValueError(f"out_dtype must be fp32, bf16 or fp16, got {out_dtype}")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, row_weights, bias)):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, row_weights, bias, out)):
         raise ValueError(f"{what} has no backward pass: call it under no_grad or detach its inputs")
     if bias is not None:
         if bias.numel() != n * N or bias.shape[-1] != N:
@@ -296,7 +296,7 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
         if t is not None and t.device != dev:
             raise ValueError(f"{name} is on {t.device}, x on {dev}")
     dtype = out_dtype or (x.dtype if out is None else out.dtype)
-    bias, act, n_out = _product_args(x, bias, activation, n, N, dtype, "mxfp4_expert_linear", row_weights)
+    bias, act, n_out = _product_args(x, bias, activation, n, N, dtype, "mxfp4_expert_linear", row_weights, out)
     if out is not None and (tuple(out.shape) != (R, n_out) or out.dtype != dtype or out.device != dev
                             or (n_out > 1 and out.stride(1) != 1) or (R > 1 and out.stride(0) < n_out)):
         raise ValueError(f"out must be [{R}, {n_out}] {dtype} on {dev} with unit inner stride")
@@ -311,4 +311,6 @@ def mxfp4_expert_linear(x: torch.Tensor, weight: MXFP4Matrix, expert_offsets: to
                 weight.data.data_ptr(), weight.sf.data_ptr(), n, N, offs.data_ptr(), _lib.ptr(gids), R, _lib.ptr(rw),
                 _lib.ptr(bias), act, ws.data_ptr(), y.data_ptr(), _lib.DTYPES[dtype], max(y.stride(0), n_out),
                 int(out is None), _lib.device_status(dev).data_ptr(), 0)
+    if out is not None:
+        torch.autograd.graph.increment_version(out)        # written in place
     return y
