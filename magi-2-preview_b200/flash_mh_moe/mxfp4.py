@@ -96,7 +96,7 @@ class MXFP4Matrix:
             packed[..., nbytes - 1] &= 15
         padded = s.new_zeros(n, rp, ka * 4)
         padded[:, :rows, :s.shape[-1]] = s
-        sf = padded.view(n, rp // 128, 4, 32, ka, 4).permute(0, 1, 4, 3, 2, 5).reshape(n, -1)
+        sf = padded.view(n, rp // 128, 4, 32, ka, 4).permute(0, 1, 4, 3, 2, 5).reshape(n, rp * ka * 4)
         return MXFP4Matrix(packed, sf.contiguous(), rows, cols, n, batched)
 
     def to_blocks(self) -> tuple[torch.Tensor, torch.Tensor]:
