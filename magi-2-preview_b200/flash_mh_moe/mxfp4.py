@@ -194,7 +194,7 @@ def _product_args(x, bias, activation, n, N, out_dtype, what, row_weights=None, 
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, row_weights, bias, out)):
         raise ValueError(f"{what} has no backward pass: call it under no_grad or detach its inputs")
     if bias is not None:
-        if bias.numel() != n * N or bias.shape[-1] != N:
+        if bias.dim() == 0 or bias.numel() != n * N or bias.shape[-1] != N:
             raise ValueError(f"bias must hold {n} x {N} values, got {tuple(bias.shape)}")
         if bias.device != x.device:
             raise ValueError(f"bias is on {bias.device}, the activations on {x.device}")
