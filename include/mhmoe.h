@@ -189,7 +189,8 @@ MHMOE_API int mhmoe_pack_weights_nvfp4(int kind, const void* w0, const void* w1,
  * grouped GEMM down x prob -> deterministic combine into y [S,H,dh] bf16.
  * R = number of routed rows, n_experts = H*E (flattened).  dh % 256 == 0,
  * de % 256 == 0.  `tok_rows`/`tok_offsets` (optional) give each (s,h) its rows
- * (row_of_flat with fixed K when tok_offsets == NULL and k_fixed > 0); when both
+ * (row_of_flat with fixed K when tok_offsets == NULL and k_fixed > 0; a negative row is
+ * an empty slot and adds nothing); when both
  * are NULL the mapping is derived from gather_ids.  workspace: see
  * mhmoe_ffn_workspace_bytes.  stage_events (optional): 5 cudaEvent_t recorded on
  * `stream` before the tile tables, before the gate/up GEMM, before the down GEMM,

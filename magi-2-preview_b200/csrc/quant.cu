@@ -198,13 +198,14 @@ __global__ void __launch_bounds__(256, MAXNB <= 3 ? 4 : 2)
   for (int j0 = 0; j0 < cnt; j0 += 32) {
     int64_t mine = -1;
     if (j0 + lane < cnt) {
+      int r = r0;
       int32_t pr = p0;
       if (j0 > 0) {
-        const int r = tok_rows[begin + j0 + lane];
+        r = tok_rows[begin + j0 + lane];
         pr = r >= 0 && r < R ? pad_of_row[r] : -1;
       }
       if (pr >= 0 && pr < rows) mine = pr;
-      if (mine < 0 && half == 0) record_error(status, MHMOE_ERR_ARGS);
+      else if (r >= 0 && half == 0) record_error(status, MHMOE_ERR_ARGS);      // < 0: an empty slot
     }
     const int n = min(32, cnt - j0);
     for (int j = 0; j < n; ++j) {
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(256)
       const int r = tok_rows[begin + j0 + sl];
       const int32_t pr = r >= 0 && r < R ? pad_of_row[r] : -1;
       if (pr >= 0 && pr < rows) mine = pr;
-      else record_error(status, MHMOE_ERR_ARGS);
+      else if (r >= 0) record_error(status, MHMOE_ERR_ARGS);                   // < 0: an empty slot
     }
     const int n = min(LPK, maxcnt - j0);
     for (int j = 0; j < n; ++j) {
