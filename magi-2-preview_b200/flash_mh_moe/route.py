@@ -282,7 +282,7 @@ def route_experts(
     selection and gets no gradient.  Forward and backward can be captured into a CUDA graph; as with
     any torch operator, no earlier autograd graph of the same leaf may be alive when a
     ``backward()`` that accumulates into it is captured (``torch.autograd.grad`` has no such
-    limit).  E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not exceed the experts of
+    limit).  H * S < 2^31, E <= 1024, K <= 32, at most 64 groups, and ``top_k`` may not exceed the experts of
     ``topk_groups`` groups (``ValueError``).
     """
     score = score_func_name2id_map.get(score_func)
@@ -293,6 +293,11 @@ def route_experts(
     _lib.require_no_tangent("route_experts", logits)
     _lib.require_cuda(logits)
     H, S, E = logits.shape
+    K, groups, keep = int(top_k), int(num_groups), int(topk_groups)
+    if not (0 < H and H * S < 1 << 31 and 0 < E <= 1024 and 0 < groups <= 64 and E % groups == 0 and 0 < keep <= groups
+            and 0 < K <= 32 and K <= keep * (E // groups)):
+        raise ValueError(f"route_experts cannot choose {K} of {E} experts in {keep} of {groups} groups for logits "
+                         f"{tuple(logits.shape)}")
     bias = mask = None
     if expert_bias is not None:
         if expert_bias.device != logits.device or expert_bias.numel() != H * E:
@@ -308,7 +313,7 @@ def route_experts(
                              f"{tuple(token_mask.shape)} {token_mask.dtype} on {token_mask.device}")
         mask = token_mask if token_mask.is_contiguous() else token_mask.contiguous()
     x = logits if E == 1 or logits.stride(2) == 1 else logits.contiguous()
-    cfg = (score, int(num_groups), int(topk_groups), int(bool(route_norm)), float(norm_eps), float(route_scale))
+    cfg = (score, groups, keep, int(bool(route_norm)), float(norm_eps), float(route_scale))
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _RouteExperts.apply(x, bias, mask, int(top_k), cfg)
-    return _route_experts(x, bias, mask, int(top_k), cfg, False)[:2]
+        return _RouteExperts.apply(x, bias, mask, K, cfg)
+    return _route_experts(x, bias, mask, K, cfg, False)[:2]
