@@ -300,8 +300,10 @@ def route_experts(
                          f"{tuple(logits.shape)}")
     bias = mask = None
     if expert_bias is not None:
-        if expert_bias.device != logits.device or expert_bias.numel() != H * E:
-            raise ValueError(f"expert_bias must hold H*E = {H * E} values on {logits.device}, got "
+        if expert_bias.device != logits.device or (
+                tuple(expert_bias.shape) != (H, E) and [d for d in expert_bias.shape if d != 1] not in (
+                    [d for d in (H * E,) if d != 1], [d for d in (H, E) if d != 1])):
+            raise ValueError(f"expert_bias must be [{H}, {E}] or [{H * E}] on {logits.device}, got "
                              f"{tuple(expert_bias.shape)} on {expert_bias.device}")
         bias = expert_bias if expert_bias.dtype == torch.float32 else expert_bias.detach().float()
         if not bias.is_contiguous():

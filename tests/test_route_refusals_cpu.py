@@ -1,4 +1,5 @@
-"""CPU: route_experts refuses sizes out of its range before it allocates or narrows them.  (Meta tensors stand for the logits: nothing is read.)"""
+"""CPU: route_experts refuses sizes out of its range before it allocates or narrows them, and biases whose layout is
+not the logits'.  (Meta tensors stand for the logits: nothing is read.)"""
 import pytest
 import torch
 
@@ -35,6 +36,13 @@ def test_sizes(shape, kw):
     from flash_mh_moe.route import route_experts
     with pytest.raises(ValueError):
         route_experts(_Logits(*shape), **kw)
+
+
+@pytest.mark.parametrize("shape", [(8, 3), (4, 6), (2, 12), (8,), ()])
+def test_bias_layout(shape):
+    from flash_mh_moe.route import route_experts
+    with pytest.raises(ValueError, match="expert_bias"):
+        route_experts(_Logits(3, 4, 8), 2, expert_bias=torch.zeros(shape, device="meta"))
 
 
 @pytest.mark.parametrize("kw", [dict(), dict(expert_bias=torch.zeros(3, 8, device="meta")), dict(num_groups=4, topk_groups=2),
