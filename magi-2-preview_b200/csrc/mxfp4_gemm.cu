@@ -280,7 +280,7 @@ __device__ __forceinline__ void mg_flat_epilogue(const MgParams& p, const MgTile
 
 // The producer and MMA warps share their schedulers with busy epilogue warps, so every
 // instruction of theirs between two asynchronous operations costs tensor time (8192^2 x 4096: a
-// loop over the stages with descriptors made on the way 120 us, this form 110; and 95 since
+// loop over the stages with descriptors made on the way 120 us, this form 110; and 91 since
 // the scale copies come from the MMA warp and the outputs leave from registers).
 // Hence: the stages are unrolled, so that barriers, descriptors and TMEM columns are constants
 // plus a base; the elected lane and the role are warp-uniform values; all 512 TMEM columns are
@@ -311,13 +311,14 @@ __device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int k
 // Wide kernel.  tmT: token rows [R, cols_p/2], box 128 B x 128; tmW: weight rows [n * N, cols_p/2], box
 // 128 B x 256.
 //
-// 8192^2 x 4096 with SwiGLU: 95 us, 5.8 PFLOP/s, bound by the MMAs and the waits between a stage's scale copies
-// and its MMAs.  131072 expert rows x 2048 x 1024 with SwiGLU: 139 us, 4.0 PFLOP/s, bound by the
-// epilogue: four stages a tile, and two special-function operations an output are at least 2048
-// clocks a tile, where the MMAs and loads alone take 107 us.
+// 8192^2 x 4096 with SwiGLU: 91 us, 6.0 PFLOP/s, bound by the MMAs and the waits between a stage's scale copies
+// and its MMAs.  131072 expert rows x 2048 x 1024 with SwiGLU: 146 us, 3.8 PFLOP/s, 4900 clocks a tile at
+// 1965 MHz.  The MMAs and loads of its four stages alone take 107 us (3600 clocks), the two
+// special-function operations an output 2048 clocks; the rest is the part of the epilogue that runs beside
+// no MMA.
 //
-// One accumulator: its 256 columns leave for registers in about 400 clocks, after which the next tile's MMAs
-// run under the epilogue.  Measured and slower (those expert rows; then 8192^2 x 4096): two
+// One accumulator: its 256 columns leave for registers in about 400 clocks, once the warps have finished the tile
+// before, and only then do the next tile's MMAs run under the epilogue.  Measured and slower (those expert rows; then 8192^2 x 4096): two
 // accumulators sharing 48 columns, the scales in two slots, 187 against 165 us, 112 against 109;
 // pairs of CTAs on one tile (cta_group::2) 252 against 199 with the grouping, 135 against 126 with the quantiser;
 // 8 epilogue warps of 128 columns 213 against 203; SwiGLU in packed pairs 214 against 156.
