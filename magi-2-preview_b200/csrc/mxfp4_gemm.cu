@@ -318,8 +318,9 @@ __device__ __forceinline__ void mg_for_stages(int t0, int total, int step, int k
 // no MMA.
 //
 // One accumulator: its 256 columns leave for registers in about 400 clocks, once the warps have finished the tile
-// before, and only then do the next tile's MMAs run under the epilogue.  Measured and slower (those expert rows; then 8192^2 x 4096): two
-// accumulators sharing 48 columns, the scales in two slots, 187 against 165 us, 112 against 109;
+// before, and only then do the next tile's MMAs run under the epilogue.  Measured and slower (those expert
+// rows; then 8192^2 x 4096): two accumulators sharing 48 columns, the scales in two slots, 187 against
+// 165 us, 112 against 109;
 // pairs of CTAs on one tile (cta_group::2) 252 against 199 with the grouping, 135 against 126 with the quantiser;
 // 8 epilogue warps of 128 columns 213 against 203; SwiGLU in packed pairs 214 against 156.
 template <int OUT, bool SWIGLU>
